@@ -114,6 +114,19 @@ SIGNATURES = {
     "ah_sample_workspace_bytes": (sz, [i32, i64]),
     "ah_sample_logits": (i32, [vp, i64, i32, i64, f32, i32, u64, i64, vp, vp, sz, vp]),
     "ah_sample_uniform": (f32, [u64, i64, i32]),
+    "ah_fp8_quantize": (i32, [vp, i64, u32, i64, i64, vp, i64, vp, i64, vp]),
+    "ah_fp8_swiglu": (i32, [vp, i64, vp, i64, u32, i64, i64, vp, i64, vp, i64, vp]),
+    "ah_fp8_add_rms_norm": (i32, [vp, i64, vp, i64, u32, vp, u32, f32, i64, i64, vp, i64, vp, i64, vp]),
+    "ah_fp8w_from_blocks": (i32, [vp, i64, vp, i64, i64, i64, C.POINTER(vp), vp]),
+    "ah_fp8w_quantize": (i32, [vp, i64, u32, i64, i64, C.POINTER(vp), vp]),
+    "ah_fp8w_from_blocks_gate_up": (i32, [vp, i64, vp, i64, vp, i64, vp, i64, i64, i64, C.POINTER(vp), vp]),
+    "ah_fp8w_quantize_gate_up": (i32, [vp, i64, vp, i64, u32, i64, i64, C.POINTER(vp), vp]),
+    "ah_fp8w_destroy": (i32, [vp]),
+    "ah_fp8w_shape": (i32, [vp, C.POINTER(i64), C.POINTER(i64)]),
+    "ah_fp8w_weight_bytes": (i64, [vp]),
+    "ah_fp8w_matmul": (i32, [vp, vp, i64, vp, i64, i64, vp, i64, u32, vp]),
+    "ah_fp8_ffn_workspace_bytes": (i32, [vp, vp, i64, C.POINTER(sz)]),
+    "ah_fp8_ffn": (i32, [vp, vp, vp, i64, vp, i64, u32, vp, u32, f32, i64, vp, i64, u32, vp, sz, vp]),
     "ah_host_gemv_4bit_into": (i32, [vp, vp, vp, vp, sz, sz, sz]),
     "ah_host_dequant_layer": (i32, [vp, vp, vp, sz, sz]),
     "ah_host_quantize": (i32, [vp, sz, sz, vp, vp]),

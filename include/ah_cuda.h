@@ -521,6 +521,76 @@ AH_API int ah_ssm_workspace_bytes(const AhSsmConfig* cfg, size_t* bytes);
 AH_API int ah_ssm_forward(const AhSsmConfig* cfg, const AhSsmWeights* w, float* conv_state, float* ssm_state,
                           const float* x, float* out, void* workspace, size_t workspace_bytes, void* stream);
 
+/* ---- 8-bit floating point projections (e4m3, scales per 128) --------------------------
+ * No reference counterpart: the reference's projections are Q4 (inference/math.rs:
+ * 255-295, inference/ffn.rs:155-174); these run the same steps of a block on
+ * weights that ship as e4m3 (1 sign, 4 exponent, 3 mantissa bits, largest 448, no
+ * infinities) in 128 x 128 blocks, with activations quantised per row and 128
+ * columns.  dtype arguments are AH_DTYPE_F32, _F16 or _BF16; row strides (ld*)
+ * count elements, columns are contiguous.  A quantised matrix is q [m][ldq]
+ * (q and ldq multiples of 16 bytes, ldq >= k; bytes past column k are neither
+ * read nor written) and scales [m][lds] f32, lds >= ceil(k / 128); element j of a
+ * row stands for q[j] * scales[j / 128].  m == 0 is a no-op.  Inputs and outputs
+ * must not overlap unless said so.
+ *
+ * With g = max(max |z|, 2^-100) over the group: q = e4m3(z * (448 / g)) rounded to
+ * nearest even, scale = g / 448.  A group that holds a NaN or an infinity stands for
+ * NaN throughout. */
+/* z = x. */
+AH_API int ah_fp8_quantize(const void* x_dev, int64_t ldx, uint32_t dtype, int64_t m, int64_t k, uint8_t* q_dev,
+                           int64_t ldq, float* scales_dev, int64_t lds, void* stream);
+/* z = silu(gate) * up, the activation of inference/ffn.rs:155-174, in f32. */
+AH_API int ah_fp8_swiglu(const void* gate_dev, int64_t ld_gate, const void* up_dev, int64_t ld_up, uint32_t dtype,
+                         int64_t m, int64_t k, uint8_t* q_dev, int64_t ldq, float* scales_dev, int64_t lds,
+                         void* stream);
+/* The residual add and inference/math.rs:53-63 rms_norm_into of a row:
+ * h = x + residual rounded to dtype and stored in residual_dev (null: h = x),
+ * r = 1 / sqrt(mean(h^2) + eps), and h * r * norm_w quantised (the group's maximum
+ * and 2^-100 are taken before the factor r: scale = g * r / 448).  norm_w_dev
+ * [k] has its own dtype.  residual_dev may be x_dev (h = 2x). */
+AH_API int ah_fp8_add_rms_norm(const void* x_dev, int64_t ldx, void* residual_dev, int64_t ldr, uint32_t dtype,
+                               const void* norm_w_dev, uint32_t norm_dtype, float eps, int64_t m, int64_t k,
+                               uint8_t* q_dev, int64_t ldq, float* scales_dev, int64_t lds, void* stream);
+
+/* Opaque device-resident weight [rows][cols]: e4m3 and one f32 scale per
+ * 128 x 128 block, in the tensor cores' tile order, on the device that was current
+ * when it was made.  The makers copy their sources, wait for `stream` and so
+ * cannot be captured. */
+typedef struct AhFp8Weight AhFp8Weight;
+/* q [rows][ldq] e4m3 bytes (any ldq >= cols), scales [ceil(rows/128)][lds >= ceil(cols/128)]. */
+AH_API int ah_fp8w_from_blocks(const uint8_t* q_dev, int64_t ldq, const float* scales_dev, int64_t lds, int64_t rows,
+                               int64_t cols, AhFp8Weight** out, void* stream);
+/* Quantises w [rows][ldw] by blocks: scale = max(max |w|, 2^-100) / 448. */
+AH_API int ah_fp8w_quantize(const void* w_dev, int64_t ldw, uint32_t dtype, int64_t rows, int64_t cols,
+                            AhFp8Weight** out, void* stream);
+/* The gate and up projections [n_ff][n_embd] of a feed-forward block as one weight
+ * of 2 * n_ff rows (gate, then up). */
+AH_API int ah_fp8w_from_blocks_gate_up(const uint8_t* gate_q_dev, int64_t ld_gate, const float* gate_scales_dev,
+                                       int64_t lds_gate, const uint8_t* up_q_dev, int64_t ld_up,
+                                       const float* up_scales_dev, int64_t lds_up, int64_t n_ff, int64_t n_embd,
+                                       AhFp8Weight** out, void* stream);
+AH_API int ah_fp8w_quantize_gate_up(const void* gate_dev, int64_t ld_gate, const void* up_dev, int64_t ld_up,
+                                    uint32_t dtype, int64_t n_ff, int64_t n_embd, AhFp8Weight** out, void* stream);
+AH_API int ah_fp8w_destroy(AhFp8Weight* w);
+AH_API int ah_fp8w_shape(const AhFp8Weight* w, int64_t* rows, int64_t* cols);
+/* Bytes a product must read of the weight (e4m3 and scales, unpadded). */
+AH_API int64_t ah_fp8w_weight_bytes(const AhFp8Weight* w);
+/* y[i][r] = sum over blocks b of 128 columns of scales[i][b] * w_scale[r / 128][b] *
+ * (sum over the block of q[i][j] * w[r][j]), sums in f32, rounded once to y_dtype:
+ * inference/math.rs:255-295 gemv_4bit_into for m tokens.  y [m][ldy], ldy >= rows. */
+AH_API int ah_fp8w_matmul(const AhFp8Weight* w, const uint8_t* q_dev, int64_t ldq, const float* scales_dev,
+                          int64_t lds, int64_t m, void* y_dev, int64_t ldy, uint32_t y_dtype, void* stream);
+/* A feed-forward block (inference/ffn.rs:72-111 with its norm, inference/mod.rs:
+ * 505-545): ah_fp8_add_rms_norm of x into residual, gate and up, silu(gate) * up
+ * quantised from f32, down: y [m][ldy] = the block's output, which the caller (or
+ * the next ah_fp8_add_rms_norm) adds to the residual.  The workspace (16-byte
+ * aligned, any contents, ah_fp8_ffn_workspace_bytes) serves one call at a time. */
+AH_API int ah_fp8_ffn_workspace_bytes(const AhFp8Weight* gate_up, const AhFp8Weight* down, int64_t m, size_t* bytes);
+AH_API int ah_fp8_ffn(const AhFp8Weight* gate_up, const AhFp8Weight* down, const void* x_dev, int64_t ldx,
+                      void* residual_dev, int64_t ldr, uint32_t dtype, const void* norm_w_dev, uint32_t norm_dtype,
+                      float eps, int64_t m, void* y_dev, int64_t ldy, uint32_t y_dtype, void* workspace_dev,
+                      size_t workspace_bytes, void* stream);
+
 /* ---- host-slice drop-ins (synchronous; reference signatures) ---------------------- */
 /* Reference: dedup/decompressor.rs:7-27 DedupCountTensor::decompress_all(&self,
  * sandbag) -> Vec<f32> (count = self.count; host arrays in, out[count]). */
