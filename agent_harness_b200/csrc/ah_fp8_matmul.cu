@@ -11,9 +11,25 @@
 #include "ah_common.cuh"
 #include "ah_fp8.cuh"
 #include "ah_sm100.cuh"
+#include "ah_tc.cuh"
+#include "ah_tma.cuh"
 
 namespace ah {
 namespace {
+
+// Tensor map of an e4m3 matrix [m][ld] read in boxes of 128 columns x box_rows
+// with the 128-byte swizzle; zero past column k and row m.
+int encode_rows(CUtensorMap* map, const void* base, uint64_t k, uint64_t m, uint64_t ld, uint32_t box_rows) {
+  auto fn = tensor_map_encoder();
+  if (!fn) return fail(AH_ECUDA, "fp8w_matmul: cuTensorMapEncodeTiled is unavailable");
+  const cuuint64_t dims[2] = {k, m}, strides[1] = {ld};
+  const cuuint32_t box[2] = {kFp8Group, box_rows}, step[2] = {1, 1};
+  const CUresult r = fn(map, CU_TENSOR_MAP_DATA_TYPE_UINT8, 2, const_cast<void*>(base), dims, strides, box, step,
+                        CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                        CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(AH_ECUDA, "fp8w_matmul: cuTensorMapEncodeTiled failed (%d)", (int)r);
+  return AH_OK;
+}
 
 // ---- building a weight ------------------------------------------------------------
 
@@ -48,7 +64,7 @@ __global__ void __launch_bounds__(256) k_fp8w_copy(const BuildArgs g) {
     int64_t row0;
     const TileSource& s = tile_source(g.s, g.gate_up, t, row0);
     const uint8_t* src = static_cast<const uint8_t*>(s.p);
-    uint8_t* dst = g.tiles + (t * g.kb + b) * kFp8TileBytes;
+    uint8_t* dst = g.tiles + fp8_image(g.gate_up, g.kb, t, b) * kFp8TileBytes;
     const bool aligned = (reinterpret_cast<uintptr_t>(src) & 15) == 0 && s.ld % 16 == 0;
     for (int i = threadIdx.x; i < kFp8TileBytes / 16; i += 256) {
       const int r = i >> 3, p = i & 7;
@@ -100,7 +116,7 @@ __global__ void __launch_bounds__(256) k_fp8w_quantize(const BuildArgs g) {
 #pragma unroll
     for (int i = 0; i < 8; ++i) a = max(a, red[i]);
     const float gm = __uint_as_float(a), inv = __fdiv_rn(kFp8Max, gm);
-    uint8_t* dst = g.tiles + (t * g.kb + b) * kFp8TileBytes;
+    uint8_t* dst = g.tiles + fp8_image(g.gate_up, g.kb, t, b) * kFp8TileBytes;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
       const int r = r0 + 32 * i;
@@ -202,55 +218,362 @@ __device__ __forceinline__ void store_y(void* y, int64_t i, uint32_t dtype, floa
   else static_cast<__nv_bfloat16*>(y)[i] = __float2bfloat16_rn(v);
 }
 
-// 64 tokens x one tile's 128 rows per CTA of 256 threads, 8 x 4 outputs each;
-// every block of 128 columns goes through shared memory as f32, 32 columns at
-// a time.
-__global__ void __launch_bounds__(256) k_fp8_matmul_simple(const MatmulArgs g) {
-  __shared__ float sa[32][64 + 1], sw[32][128 + 1];
-  const int64_t t = blockIdx.x, m0 = (int64_t)blockIdx.y * 64;
-  const int tx = threadIdx.x & 31, ty = threadIdx.x >> 5;  // rows tx + 32 * j, tokens ty + 8 * i
-  float acc[8][4] = {};
-  for (int64_t b = 0; b < g.kb; ++b) {
-    const uint8_t* tile = g.tiles + (t * g.kb + b) * kFp8TileBytes;
-    float part[8][4] = {};
-    for (int c0 = 0; c0 < 128; c0 += 32) {
-      __syncthreads();
-      for (int i = threadIdx.x; i < 64 * 32; i += 256) {
-        const int tok = i >> 5, c = i & 31;
-        const int64_t col = b * kFp8Group + c0 + c;
-        sa[c][tok] = m0 + tok < g.m && col < g.cols ? e4m3x2_f32(g.a[(m0 + tok) * g.lda + col]).x : 0.0f;
-      }
-      for (int i = threadIdx.x; i < 128 * 32; i += 256) {
-        const int r = i >> 5, c = c0 + (i & 31);
-        sw[i & 31][r] = e4m3x2_f32(tile[r * 128 + (((c >> 4) ^ (r & 7)) << 4) + (c & 15)]).x;
-      }
-      __syncthreads();
-      for (int c = 0; c < 32; ++c)
-#pragma unroll
-        for (int i = 0; i < 8; ++i)
-#pragma unroll
-          for (int j = 0; j < 4; ++j) part[i][j] = fmaf(sa[c][ty + 8 * i], sw[c][tx + 32 * j], part[i][j]);
+// ---- few tokens: weight rows on the MMA's M, tokens on N ------------------------------
+//
+// A CTA takes one 128-row tile (or a gate/up pair of tiles) and a run of its
+// column blocks for kNt tokens; a cluster of up to 8 CTAs shares a tile's column
+// blocks and adds its members' sums through distributed shared memory in rank
+// order.
+//
+//   warp 0     producer: one bulk copy of KS column blocks of weights per stage
+//              (contiguous, 16 or 32 KB each) and a TMA box of each block's tokens
+//   warp 1     TMEM owner, MMA issuer: M = 128, N = kNt, K = 32, four per block
+//   warps 2-5  a block's sums from tensor memory, times a_scale * w_scale, added
+//              to f32 registers; then the cluster's sum and the output
+//
+// A block's sums are overwritten, not accumulated, in tensor memory: the scales
+// change with every block.  kBufs buffers let the MMAs run ahead of the readers.
+//
+// Bound by the weight stream: the first stages' weights are requested before the
+// kernel waits for the grid ahead of it (a weight is complete once its handle
+// exists).
+
+constexpr uint32_t kWaitLimit = 1u << 24;
+constexpr int kSmallThreads = 192;
+constexpr int kScaleBlocks = 8;  // column blocks whose scales are staged together
+
+template <int kNt, bool kGlu>
+struct Small {
+  static constexpr int kTiles = kGlu ? 2 : 1;
+  static constexpr int kKs = !kGlu && kNt == 16 ? 2 : 1;  // column blocks per stage
+  static constexpr int kBlockBytes = kTiles * kFp8TileBytes;
+  static constexpr int kActBytes = kNt * kFp8Group;
+  static constexpr int kStageBytes = kKs * (kBlockBytes + kActBytes);
+  static constexpr int kCols = kNt * kTiles;  // TMEM columns of one buffer
+  static constexpr int kScaleBytes = 2 * kScaleBlocks * kCols * 4;
+  static constexpr int kBudget = 113 * 1024 - 1024 - 512;  // two CTAs per SM, barriers, 1 KB alignment
+  static constexpr int kStages = (kBudget - kScaleBytes) / kStageBytes;
+  static constexpr int kBufs = kCols <= 64 ? 4 : 2;
+  static constexpr int kTmemCols = kCols * kBufs < 32 ? 32 : kCols * kBufs;
+  static_assert(kTmemCols <= 256, "two CTAs share an SM's 512 tensor-memory columns");
+  static_assert(kStages >= 2, "at least two stages");
+  // the sums [kCols][128] go over the idle ring for the cluster's reduction
+  static_assert(kCols * 128 * 4 <= kStages * kStageBytes, "partial sums must fit the ring");
+  static constexpr int kScale = kStages * kStageBytes;
+  static constexpr int kBars = kScale + kScaleBytes;
+  static constexpr int kMisc = kBars + (2 * kStages + 2 * kBufs + 1) * 8;
+  static constexpr int kTotal = kMisc + 16;
+  static constexpr size_t kDynamic = (size_t)kTotal + 1024;  // slack for 1 KB alignment
+  static_assert(kDynamic <= 113 * 1024, "two CTAs per SM");
+};
+
+struct SmallArgs {
+  CUtensorMap tm_a;  // e4m3 activations [m][cols], box 128 x kNt, 128-byte swizzle
+  MatmulArgs g;
+  uint8_t* act_q;    // SwiGLU: output instead of y
+  int64_t ld_act;
+  float* act_scales;
+  int64_t lds_act;
+  int* err;
+};
+
+// Waits on `bar`'s phase `parity`; on give-up raises the CTA's abort flag.
+__device__ __forceinline__ bool wait_or_abort(uint64_t* bar, uint32_t parity, int* err, volatile int* abort_flag) {
+  if (mbar_wait_bounded(bar, parity, err, AH_ETIMEOUT, kWaitLimit)) return true;
+  *abort_flag = 1;
+  return false;
+}
+
+__device__ __forceinline__ void promote_barrier() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
+
+template <int kNt, bool kGlu>
+__global__ void __launch_bounds__(kSmallThreads, 2) k_fp8_small(const __grid_constant__ SmallArgs p) {
+  using L = Small<kNt, kGlu>;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + L::kBars);
+  uint64_t* empty = full + L::kStages;
+  uint64_t* d_full = empty + L::kStages;
+  uint64_t* d_empty = d_full + L::kBufs;
+  uint64_t* drained = d_empty + L::kBufs;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + L::kMisc);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + L::kMisc + 4);
+  const MatmulArgs& g = p.g;
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int nc = (int)gridDim.x, rank = (int)blockIdx.x;  // the cluster spans x
+  const int64_t unit = blockIdx.y;                        // tile, or gate/up pair
+  const int64_t m0 = (int64_t)blockIdx.z * kNt;
+  const int64_t b0 = g.kb * rank / nc, b1 = g.kb * (rank + 1) / nc;
+  const int nb = (int)(b1 - b0);
+  const int n_stage = (nb + L::kKs - 1) / L::kKs;
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < L::kStages; ++i) {
+      mbar_init(&full[i], 1);
+      mbar_init(&empty[i], 1);
     }
-    const float ws = g.wscales[t * g.kb + b];
+    for (int i = 0; i < L::kBufs; ++i) {
+      mbar_init(&d_full[i], 1);
+      mbar_init(&d_empty[i], 4);
+    }
+    mbar_init(drained, 1);
+    *abort_flag = 0;
+    fence_mbar_init();
+  }
+  if (warp == 1) tmem_alloc(tmem_slot, L::kTmemCols);
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  // after the allocation: a dependent grid's CTA on this SM must not take the
+  // tensor memory first and then wait for this grid
+  pdl_launch_dependents();
+  const uint32_t tmem = *tmem_slot;
+
+  if (warp == 0) {
+    if (lane == 0) {
+      const uint8_t* src = g.tiles + fp8_image(g.gate_up, g.kb, unit * L::kTiles, b0) * kFp8TileBytes;
+      const bool halves = !kGlu && g.gate_up;  // one of a pair's two images per column block
+      auto blocks = [&](int s) { return min(L::kKs, nb - s * L::kKs); };
+      auto weights = [&](int s) {
+        const int r = s % L::kStages, n = blocks(s);
+        mbar_arrive_expect_tx(&full[r], (uint32_t)(n * (L::kBlockBytes + L::kActBytes)));
+        uint8_t* dst = smem + r * L::kStageBytes;
+        if (!halves)
+          bulk_g2s(dst, src + (size_t)s * L::kKs * L::kBlockBytes, (uint32_t)(n * L::kBlockBytes), &full[r]);
+        else
+          for (int i = 0; i < n; ++i)
+            bulk_g2s(dst + i * kFp8TileBytes, src + (size_t)(s * L::kKs + i) * 2 * kFp8TileBytes, kFp8TileBytes,
+                     &full[r]);
+      };
+      auto tokens = [&](int s) {
+        const int r = s % L::kStages;
+        uint8_t* dst = smem + r * L::kStageBytes + L::kKs * L::kBlockBytes;
+        for (int i = 0; i < blocks(s); ++i)
+          tma_load_2d(dst + i * L::kActBytes, &p.tm_a, (int)(b0 + s * L::kKs + i) * kFp8Group, (int)m0, &full[r]);
+      };
+      const int ahead = min(n_stage, L::kStages);
+      for (int s = 0; s < ahead; ++s) weights(s);
+      pdl_wait();  // the tokens come from the preceding grid
+      for (int s = 0; s < ahead; ++s) tokens(s);
+      int issued = ahead;
+      for (int s = ahead; s < n_stage; ++s) {
+        if (*abort_flag ||
+            !wait_or_abort(&empty[s % L::kStages], (uint32_t)((s / L::kStages - 1) & 1), p.err, abort_flag))
+          break;
+        weights(s);
+        tokens(s);
+        ++issued;
+      }
+      if (*abort_flag)  // the copies in flight land before the CTA can exit
+        for (int s = max(0, issued - L::kStages); s < issued; ++s)
+          mbar_wait_bounded(&full[s % L::kStages], (uint32_t)((s / L::kStages) & 1), p.err, AH_ETIMEOUT, kWaitLimit);
+    }
+  } else if (warp == 1) {
+    if (lane == 0) {
+      constexpr uint32_t idesc = idesc_e4m3(128, kNt);
+      for (int i = 0; i < nb; ++i) {
+        const int s = i / L::kKs, r = s % L::kStages, buf = i % L::kBufs;
+        if (*abort_flag) break;
+        if (i % L::kKs == 0 && !wait_or_abort(&full[r], (uint32_t)((s / L::kStages) & 1), p.err, abort_flag)) break;
+        if (i >= L::kBufs && !wait_or_abort(&d_empty[buf], (uint32_t)((i / L::kBufs - 1) & 1), p.err, abort_flag))
+          break;
+        tc_fence_after();
+        const uint32_t st = smem_u32(smem + r * L::kStageBytes);
+        const uint32_t wb = st + (i % L::kKs) * L::kBlockBytes;
+        const uint64_t bdesc = sw128_desc(st + L::kKs * L::kBlockBytes + (i % L::kKs) * L::kActBytes);
 #pragma unroll
-    for (int i = 0; i < 8; ++i) {
-      const int64_t tok = m0 + ty + 8 * i;
-      const float s = tok < g.m ? g.ascales[tok * g.lds + b] * ws : 0.0f;
+        for (int h = 0; h < L::kTiles; ++h) {
+          const uint64_t adesc = sw128_desc(wb + h * kFp8TileBytes);
 #pragma unroll
-      for (int j = 0; j < 4; ++j) acc[i][j] = fmaf(s, part[i][j], acc[i][j]);
+          for (int kk = 0; kk < 4; ++kk)
+            mma_f8(tmem + buf * L::kCols + h * kNt, adesc + kk * 2, bdesc + kk * 2, idesc, kk > 0);
+        }
+        if (i % L::kKs == L::kKs - 1 || i == nb - 1) mma_commit(&empty[r]);
+        mma_commit(&d_full[buf]);
+      }
+      if (*abort_flag) {  // the MMAs in flight end before the tensor memory is freed
+        mma_commit(drained);
+        mbar_wait_bounded(drained, 0, p.err, AH_ETIMEOUT, kWaitLimit);
+      }
+    }
+  } else {
+    const int q = warp & 3, t = threadIdx.x - 64;  // TMEM lane quarter, reader index
+    float* sc = reinterpret_cast<float*>(smem + L::kScale);  // [2][kScaleBlocks][kCols]
+    constexpr int kPer = kScaleBlocks * L::kCols / 128;
+    float next[kPer];
+    // thread t's share of the scale products of blocks [i0, i0 + kScaleBlocks):
+    // neighbouring threads take neighbouring blocks of a token
+    auto fetch = [&](int i0) {
+#pragma unroll
+      for (int j = 0; j < kPer; ++j) {
+        const int e = t + j * 128, i = i0 + e % kScaleBlocks, c = e / kScaleBlocks;
+        const int64_t tok = m0 + c % kNt;
+        next[j] = i < nb && tok < g.m ? g.ascales[tok * g.lds + b0 + i] *
+                                            g.wscales[(unit * L::kTiles + c / kNt) * g.kb + b0 + i]
+                                      : 0.0f;
+      }
+    };
+    pdl_wait();  // the scales come from the preceding grid
+    fetch(0);
+    float acc[L::kCols];
+#pragma unroll
+    for (int j = 0; j < L::kCols; ++j) acc[j] = 0.0f;
+    bool ok = true;
+    for (int i = 0; i < nb; ++i) {
+      const int buf = i % L::kBufs;
+      float* set = sc + (i / kScaleBlocks & 1) * kScaleBlocks * L::kCols;
+      if (i % kScaleBlocks == 0) {
+#pragma unroll
+        for (int j = 0; j < kPer; ++j) {
+          const int e = t + j * 128;
+          set[e % kScaleBlocks * L::kCols + e / kScaleBlocks] = next[j];
+        }
+        // also: every reader is done with the set before last
+        promote_barrier();
+        fetch(i + kScaleBlocks);
+      }
+      if (lane == 0)
+        ok = !*abort_flag && wait_or_abort(&d_full[buf], (uint32_t)((i / L::kBufs) & 1), p.err, abort_flag);
+      ok = __shfl_sync(0xFFFFFFFFu, ok, 0);
+      if (ok) {
+        tc_fence_after();
+        const float* s = set + i % kScaleBlocks * L::kCols;
+        const uint32_t ta = tmem + ((uint32_t)(q * 32) << 16) + buf * L::kCols;
+        constexpr int kStep = L::kCols < 32 ? 16 : 32;
+#pragma unroll
+        for (int c = 0; c < L::kCols; c += kStep) {
+          float v[kStep];
+          if constexpr (kStep == 16) tmem_ld16(ta + c, v);
+          else tmem_ld32(ta + c, v);
+#pragma unroll
+          for (int j = 0; j < kStep; j += 4) {
+            const float4 f = *reinterpret_cast<const float4*>(s + c + j);
+            acc[c + j] = fmaf(v[j], f.x, acc[c + j]);
+            acc[c + j + 1] = fmaf(v[j + 1], f.y, acc[c + j + 1]);
+            acc[c + j + 2] = fmaf(v[j + 2], f.z, acc[c + j + 2]);
+            acc[c + j + 3] = fmaf(v[j + 3], f.w, acc[c + j + 3]);
+          }
+        }
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&d_empty[buf]);
+      }
+    }
+    // every block's MMAs have read their stages: the ring is idle
+    float* part = reinterpret_cast<float*>(smem);  // [kCols][128]
+#pragma unroll
+    for (int c = 0; c < L::kCols; ++c) part[c * 128 + q * 32 + lane] = acc[c];
+  }
+
+  __syncwarp();
+  __syncthreads();
+  cluster_arrive();
+  cluster_wait();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc(tmem, L::kTmemCols);
+  }
+  const int live = (int)(g.m - m0 < kNt ? g.m - m0 : kNt);
+  if (warp >= 2 && !*abort_flag) {
+    const int t = threadIdx.x - 64;
+    const uint32_t part = smem_u32(smem);
+    if constexpr (kGlu) {
+      // one warp per token: 4 rows per lane, the group's maximum over the warp
+      const int64_t n_ff = g.rows / 2, r = unit * kFp8Group + lane * 4;
+      for (int c = rank + (warp - 2) * nc; c < live; c += 4 * nc) {
+        float gt[4] = {}, up[4] = {};
+        for (int k = 0; k < nc; ++k) {
+          const uint32_t peer = mapa_shared(part, k) + lane * 16;
+          const uint4 a = ld_dsmem_v4(peer + c * 512), b = ld_dsmem_v4(peer + (kNt + c) * 512);
+          gt[0] += __uint_as_float(a.x); gt[1] += __uint_as_float(a.y);
+          gt[2] += __uint_as_float(a.z); gt[3] += __uint_as_float(a.w);
+          up[0] += __uint_as_float(b.x); up[1] += __uint_as_float(b.y);
+          up[2] += __uint_as_float(b.z); up[3] += __uint_as_float(b.w);
+        }
+        uint32_t mx = __float_as_uint(kFp8Tiny);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          gt[i] = r + i < n_ff ? fp8_silu_mul(gt[i], up[i]) : 0.0f;
+          mx = max(mx, __float_as_uint(gt[i]) & 0x7FFFFFFFu);
+        }
+        const float gm = __uint_as_float(__reduce_max_sync(0xFFFFFFFFu, mx)), inv = __fdiv_rn(kFp8Max, gm);
+        const uint32_t w = cvt_e4m3x4(gt[0] * inv, gt[1] * inv, gt[2] * inv, gt[3] * inv);
+        uint8_t* qrow = p.act_q + (m0 + c) * p.ld_act + r;  // ld_act is a multiple of 16
+        if (r + 4 <= n_ff) *reinterpret_cast<uint32_t*>(qrow) = w;
+        else
+          for (int i = 0; i < 4 && r + i < n_ff; ++i) qrow[i] = (uint8_t)(w >> (8 * i));
+        if (lane == 0) p.act_scales[(m0 + c) * p.lds_act + unit] = gm * (1.0f / kFp8Max);
+      }
+    } else {
+      const int64_t rows = g.gate_up ? g.rows / 2 : g.rows;  // rows of the tile's source
+      const int64_t r0 = (g.gate_up ? unit >> 1 : unit) * kFp8Group, out0 = g.gate_up && (unit & 1) ? rows : 0;
+      // (token, row) elements over the cluster's readers, rows fastest
+      for (int e = rank * 128 + t; e < live * 128; e += nc * 128) {
+        float v = 0.0f;
+        for (int k = 0; k < nc; ++k) v += ld_dsmem_f32(mapa_shared(part, k) + e * 4);
+        const int64_t r = r0 + (e & 127);
+        if (r < rows) store_y(g.y, (m0 + (e >> 7)) * g.ldy + out0 + r, g.y_dtype, v);
+      }
     }
   }
-  // tile t's first output column and the rows of its source
-  const int64_t rows = g.gate_up ? g.rows / 2 : g.rows;
-  const int64_t r0 = (g.gate_up ? t >> 1 : t) * kFp8Group;
-  const int64_t out0 = g.gate_up && (t & 1) ? rows : 0;
-#pragma unroll
-  for (int i = 0; i < 8; ++i)
-#pragma unroll
-    for (int j = 0; j < 4; ++j) {
-      const int64_t tok = m0 + ty + 8 * i, r = r0 + tx + 32 * j;
-      if (tok < g.m && r < rows) store_y(g.y, tok * g.ldy + out0 + r, g.y_dtype, acc[i][j]);
-    }
+  // the other members have read this CTA's sums
+  __syncwarp();
+  cluster_arrive();
+  cluster_wait();
+}
+
+// CTAs that share a tile's column blocks: as many as keep two CTAs per SM
+// busy, each with two column blocks at least.
+int small_cluster(int64_t units, int64_t kb) {
+  int c = 1;
+  while (c < 8 && units * c * 2 <= 2 * sm_count() && kb >= 4 * c) c *= 2;
+  return c;
+}
+
+template <int kNt, bool kGlu>
+int launch_small(SmallArgs& p, cudaStream_t st) {
+  using L = Small<kNt, kGlu>;
+  const MatmulArgs& g = p.g;
+  int rc = encode_rows(&p.tm_a, g.a, (uint64_t)g.cols, (uint64_t)g.m, (uint64_t)g.lda, kNt);
+  if (rc != AH_OK) return rc;
+  static std::once_flag once[64];
+  static cudaError_t attr[64];
+  int dev = 0;
+  AH_CUDA_TRY(cudaGetDevice(&dev));
+  AH_REQUIRE(dev < 64, "fp8w_matmul: device %d out of range", dev);
+  std::call_once(once[dev], [&] {
+    attr[dev] = cudaFuncSetAttribute(k_fp8_small<kNt, kGlu>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                     (int)L::kDynamic);
+  });
+  AH_CUDA_TRY(attr[dev]);
+  const int64_t units = g.nt / L::kTiles, z = (g.m + kNt - 1) / kNt;
+  AH_REQUIRE(units <= 65535 && z <= 65535, "fp8w_matmul: more than 65535 row or token tiles");
+  const int c = small_cluster(units * z, g.kb);
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)c, (unsigned)units, (unsigned)z);
+  cfg.blockDim = dim3(kSmallThreads);
+  cfg.dynamicSmemBytes = L::kDynamic;
+  cfg.stream = st;
+  cudaLaunchAttribute at[2];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  at[1].id = cudaLaunchAttributeClusterDimension;
+  at[1].val.clusterDim.x = (unsigned)c;
+  at[1].val.clusterDim.y = 1;
+  at[1].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 2;
+  AH_CUDA_TRY(cudaLaunchKernelEx(&cfg, k_fp8_small<kNt, kGlu>, (const SmallArgs)p));
+  return AH_OK;
+}
+
+template <bool kGlu>
+int dispatch_small(SmallArgs& p, cudaStream_t st) {
+  if (p.g.m <= 16) return launch_small<16, kGlu>(p, st);
+  if (p.g.m <= 32) return launch_small<32, kGlu>(p, st);
+  if (kGlu || p.g.m <= 64) return launch_small<64, kGlu>(p, st);
+  if constexpr (!kGlu) return launch_small<128, false>(p, st);
 }
 
 int check_device(const char* who, const AhFp8Weight* w) {
@@ -275,32 +598,43 @@ int matmul(const AhFp8Weight* w, const uint8_t* q, int64_t ldq, const float* sca
   if (rc != AH_OK) return rc;
   const MatmulArgs g{w->tiles, w->scales, w->rows, w->cols, w->nt, w->kb, w->gate_up, q, ldq, scales, lds, m, y, ldy,
                      y_dtype};
-  AH_REQUIRE((m + 63) / 64 <= 65535, "fp8w_matmul: m too large for one launch");
-  k_fp8_matmul_simple<<<dim3((unsigned)w->nt, (unsigned)((m + 63) / 64)), 256, 0, st>>>(g);
-  AH_LAUNCH_CHECK();
-  return AH_OK;
+  SmallArgs p{};
+  p.g = g;
+  p.err = device_error_word();
+  return dispatch_small<false>(p, st);
+}
+
+// silu(gate) * up of the products with a gate/up weight, quantised from f32.
+int matmul_swiglu(const AhFp8Weight* w, const uint8_t* q, int64_t ldq, const float* scales, int64_t lds, int64_t m,
+                  uint8_t* act_q, int64_t ld_act, float* act_scales, int64_t lds_act, cudaStream_t st) {
+  SmallArgs p{};
+  p.g = MatmulArgs{w->tiles, w->scales, w->rows, w->cols, w->nt, w->kb, true, q, ldq, scales, lds, m, nullptr, 0, 0};
+  p.act_q = act_q;
+  p.ld_act = ld_act;
+  p.act_scales = act_scales;
+  p.lds_act = lds_act;
+  p.err = device_error_word();
+  return dispatch_small<true>(p, st);
 }
 
 // ---- the feed-forward block ----------------------------------------------------------
 
-// Workspace: the norm's q and scales, gate | up in f32, the activation's q and scales.
+// Workspace: the norm's q and scales, the activation's q and scales.
 struct FfnLayout {
-  int64_t ldq1, lds1, n_ff, ldq2, lds2;
-  size_t q1, s1, gu, q2, s2, total;
+  int64_t ldq1, lds1, ldq2, lds2;
+  size_t q1, s1, q2, s2, total;
 };
 
 FfnLayout ffn_layout(const AhFp8Weight* gu, const AhFp8Weight* down, int64_t m) {
   auto up = [](size_t v) { return (v + 255) / 256 * 256; };
   FfnLayout l;
-  l.n_ff = gu->rows / 2;
   l.ldq1 = (gu->cols + 15) / 16 * 16;
   l.lds1 = gu->kb;
-  l.ldq2 = (l.n_ff + 15) / 16 * 16;
+  l.ldq2 = (down->cols + 15) / 16 * 16;
   l.lds2 = down->kb;
   l.q1 = 0;
   l.s1 = l.q1 + up((size_t)m * l.ldq1);
-  l.gu = l.s1 + up((size_t)m * l.lds1 * 4);
-  l.q2 = l.gu + up((size_t)m * gu->rows * 4);
+  l.q2 = l.s1 + up((size_t)m * l.lds1 * 4);
   l.s2 = l.q2 + up((size_t)m * l.ldq2);
   l.total = l.s2 + up((size_t)m * l.lds2 * 4);
   return l;
@@ -393,14 +727,10 @@ int ah_fp8_ffn(const AhFp8Weight* gate_up, const AhFp8Weight* down, const void* 
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   uint8_t *q1 = ws + l.q1, *q2 = ws + l.q2;
   float *s1 = reinterpret_cast<float*>(ws + l.s1), *s2 = reinterpret_cast<float*>(ws + l.s2);
-  float* gu = reinterpret_cast<float*>(ws + l.gu);
   rc = ah_fp8_add_rms_norm(x, ldx, residual, ldr, dtype, norm_w, norm_dtype, eps, m, gate_up->cols, q1, l.ldq1, s1,
                            l.lds1, stream);
   if (rc != AH_OK) return rc;
-  rc = ah_fp8w_matmul(gate_up, q1, l.ldq1, s1, l.lds1, m, gu, gate_up->rows, AH_DTYPE_F32, stream);
-  if (rc != AH_OK) return rc;
-  rc = ah_fp8_swiglu(gu, gate_up->rows, gu + l.n_ff, gate_up->rows, AH_DTYPE_F32, m, l.n_ff, q2, l.ldq2, s2, l.lds2,
-                     stream);
+  rc = matmul_swiglu(gate_up, q1, l.ldq1, s1, l.lds1, m, q2, l.ldq2, s2, l.lds2, as_stream(stream));
   if (rc != AH_OK) return rc;
   return ah_fp8w_matmul(down, q2, l.ldq2, s2, l.lds2, m, y, ldy, y_dtype, stream);
 }
