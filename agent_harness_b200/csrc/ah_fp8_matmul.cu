@@ -5,6 +5,7 @@
 //
 // b runs over the blocks of 128 columns.  The inner sums are exact products
 // summed in f32; the scales multiply each block's sum in f32.
+#include <algorithm>
 #include <mutex>
 #include <new>
 
@@ -523,6 +524,12 @@ __global__ void __launch_bounds__(kSmallThreads, 2) k_fp8_small(const __grid_con
   cluster_wait();
 }
 
+int device_once(int* dev) {
+  AH_CUDA_TRY(cudaGetDevice(dev));
+  AH_REQUIRE(*dev >= 0 && *dev < 64, "fp8w_matmul: device %d out of range", *dev);
+  return AH_OK;
+}
+
 // CTAs that share a tile's column blocks: as many as keep two CTAs per SM
 // busy, each with two column blocks at least.
 int small_cluster(int64_t units, int64_t kb) {
@@ -540,8 +547,8 @@ int launch_small(SmallArgs& p, cudaStream_t st) {
   static std::once_flag once[64];
   static cudaError_t attr[64];
   int dev = 0;
-  AH_CUDA_TRY(cudaGetDevice(&dev));
-  AH_REQUIRE(dev < 64, "fp8w_matmul: device %d out of range", dev);
+  rc = device_once(&dev);
+  if (rc != AH_OK) return rc;
   std::call_once(once[dev], [&] {
     attr[dev] = cudaFuncSetAttribute(k_fp8_small<kNt, kGlu>, cudaFuncAttributeMaxDynamicSharedMemorySize,
                                      (int)L::kDynamic);
@@ -576,6 +583,382 @@ int dispatch_small(SmallArgs& p, cudaStream_t st) {
   if constexpr (!kGlu) return launch_small<128, false>(p, st);
 }
 
+// ---- many tokens: CTA pairs, 256 tokens x 256 weight rows ---------------------------------
+//
+// A persistent pair walks tiles of 256 tokens x two weight tiles (a gate/up pair
+// for SwiGLU).  Each CTA loads its 128 tokens and one of the two weight images of
+// a column block (32 KB) and holds all 256 columns of its tokens' sums:
+//
+//   warp 0     producer (both CTAs, all copies complete on the leader's barrier)
+//   warp 1     TMEM owner; in the leader the MMA issuer: cta_group::2, M = 256,
+//              N = 256, K = 32, four per column block into one of two buffers of
+//              256 tensor-memory columns
+//   warps 4-11 a thread owns one token (tensor-memory lane) and 64 columns of each
+//              weight tile: sums times a_scale * w_scale into 128 f32 registers,
+//              one multiply-add each, since w_scale is one number per weight tile
+//              and column block; then the tile's output
+//
+// Both CTAs read half of B from each other's shared memory, so a pair moves
+// 64 KB per column block for 512 x 128 operand columns where two single CTAs of
+// 128 x 256 would move 96 KB.
+
+constexpr int kBigStages = 6;
+constexpr int kBigThreads = 384;
+// Registers: 384 threads start with 168 each (64512); the first four warps drop
+// to 40 and the eight readers rise to 232 (128 * 40 + 256 * 232 = 64512).
+constexpr int kBigRegsFew = 40, kBigRegsMany = 232;
+constexpr int kBigTokens = 256;
+
+struct Big {
+  static constexpr int kStageBytes = 2 * kFp8TileBytes;  // 128 tokens, one weight image
+  static constexpr int kStage = kBigStages * kStageBytes;  // output staging: 4 KB per reader warp
+  static constexpr int kMax = kStage + 8 * 4096;           // SwiGLU: group maxima [2][128]
+  static constexpr int kBars = kMax + 1024;
+  static constexpr int kMisc = kBars + (2 * kBigStages + 4 + 1) * 8;
+  static constexpr int kTotal = kMisc + 16;
+  static constexpr size_t kDynamic = (size_t)kTotal + 1024;
+  static_assert(kDynamic <= 227 * 1024, "one CTA per SM");
+};
+
+struct BigArgs {
+  CUtensorMap tm_a;  // e4m3 activations [m][cols], box 128 x 128, 128-byte swizzle
+  CUtensorMap tm_w;  // weight images as bytes [images * 128][128], box 128 x 128
+  CUtensorMap tm_y;  // y [m][rows], box 128 bytes x 32 rows, 128-byte swizzle (when y_map)
+  MatmulArgs g;
+  bool y_map;
+  uint8_t* act_q;
+  int64_t ld_act;
+  float* act_scales;
+  int64_t lds_act;
+  int* err;
+};
+
+// Four consecutive column blocks' scales of one row, from block b (zero past kb).
+__device__ __forceinline__ void load_scales4(const float* row, int b, int kb, bool vec, float (&v)[4]) {
+  if (vec && b + 4 <= kb) {
+    const float4 f = *reinterpret_cast<const float4*>(row + b);
+    v[0] = f.x; v[1] = f.y; v[2] = f.z; v[3] = f.w;
+  } else {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) v[i] = b + i < kb ? row[b + i] : 0.0f;
+  }
+}
+
+// silu(g) * u with the fast exponential and division: the product is rounded to
+// 4 significant bits next, a relative error of about 2^-20 moves one in 10^5.
+__device__ __forceinline__ float fp8_silu_mul_fast(float g, float u) { return __fdividef(g, 1.0f + __expf(-g)) * u; }
+
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float a, float b);
+template <>
+__device__ __forceinline__ uint32_t pack2<__half>(float a, float b) {
+  const __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+template <>
+__device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float a, float b) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+template <bool kGlu>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kBigThreads, 1) k_fp8_big(const __grid_constant__ BigArgs p) {
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + Big::kBars);  // the leader's are used
+  uint64_t* empty = full + kBigStages;
+  uint64_t* d_full = empty + kBigStages;
+  uint64_t* d_empty = d_full + 2;  // the leader's are used
+  uint64_t* drained = d_empty + 2;
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + Big::kMisc);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + Big::kMisc + 4);
+  const MatmulArgs& g = p.g;
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int rank = (int)cluster_ctarank();
+  const int mt = (int)((g.m + kBigTokens - 1) / kBigTokens), nt = (int)g.nt, kb = (int)g.kb;
+  const int tiles = mt * ((nt + 1) / 2), first = blockIdx.x / 2, step = gridDim.x / 2;
+
+  if (threadIdx.x == 0) {
+    for (int i = 0; i < kBigStages; ++i) {
+      mbar_init(&full[i], 1);
+      mbar_init(&empty[i], 1);
+    }
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(&d_full[i], 1);
+      mbar_init(&d_empty[i], 16);  // eight reader warps in each CTA
+    }
+    mbar_init(drained, 1);
+    *abort_flag = 0;
+    fence_mbar_init();
+  }
+  if (warp == 1) tmem_alloc_pair(tmem_slot, 512);
+  tc_fence_before();
+  __syncthreads();
+  cluster_arrive();
+  cluster_wait();
+  tc_fence_after();
+  pdl_launch_dependents();  // after the allocation, as in k_fp8_small
+  const uint32_t tmem = *tmem_slot;
+
+  if (warp < 4) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kBigRegsFew));
+    if (threadIdx.x == 0) {
+      // a stage's copies land in both CTAs and complete on the leader's barrier
+      const uint32_t full0 = mapa_shared(smem_u32(full), 0), st0 = smem_u32(smem);
+      auto weights = [&](int s, int tile, int b) {
+        if (rank == 0) mbar_arrive_expect_tx(&full[s], 2 * Big::kStageBytes);
+        const int t = min(tile / mt * 2 + rank, nt - 1);  // past an odd last tile: read again, not stored
+        tma_load_2d_pair(st0 + s * Big::kStageBytes + kFp8TileBytes, &p.tm_w, 0,
+                         (int)fp8_image(g.gate_up, kb, t, b) * kFp8Group, full0 + s * 8);
+      };
+      const int ahead = min(kb, kBigStages);
+      for (int i = 0; i < ahead; ++i) weights(i, first, i);
+      pdl_wait();  // the tokens come from the preceding grid
+      int s = 0, left = ahead, round = 0;  // stage, blocks whose weights are under way, passes over the ring
+      for (int tile = first; tile < tiles && !*abort_flag; tile += step) {
+        const int row = tile % mt * kBigTokens + rank * 128;
+        for (int b = 0; b < kb; ++b) {
+          if (round > 0 &&
+              (*abort_flag || !wait_or_abort(&empty[s], (uint32_t)((round - 1) & 1), p.err, abort_flag)))
+            break;
+          if (left > 0) --left;
+          else weights(s, tile, b);
+          tma_load_2d_pair(st0 + s * Big::kStageBytes, &p.tm_a, b * kFp8Group, row, full0 + s * 8);
+          if (++s == kBigStages) {
+            s = 0;
+            ++round;
+          }
+        }
+      }
+      if (*abort_flag && rank == 0)  // the copies in flight land before the pair can exit
+        for (int i = 0; i < kBigStages; ++i)
+          if (i < s || round > 0)
+            mbar_wait_bounded(&full[i], (uint32_t)((i < s ? round : round - 1) & 1), p.err, AH_ETIMEOUT, kWaitLimit);
+    } else if (threadIdx.x == 32 && rank == 0) {
+      constexpr uint32_t idesc = idesc_e4m3(256, 256);
+      int s = 0, n = 0;
+      uint32_t ph = 0;
+      for (int tile = first; tile < tiles && !*abort_flag; tile += step)
+        for (int b = 0; b < kb; ++b, ++n) {
+          const int buf = n & 1;
+          if (*abort_flag || !wait_or_abort(&full[s], ph, p.err, abort_flag)) break;
+          if (n >= 2 && !wait_or_abort(&d_empty[buf], (uint32_t)((n / 2 - 1) & 1), p.err, abort_flag)) break;
+          tc_fence_after();
+          const uint32_t st = smem_u32(smem + s * Big::kStageBytes);
+          const uint64_t adesc = sw128_desc(st), bdesc = sw128_desc(st + kFp8TileBytes);
+#pragma unroll
+          for (int kk = 0; kk < 4; ++kk) mma_f8_pair(tmem + buf * 256, adesc + kk * 2, bdesc + kk * 2, idesc, kk > 0);
+          mma_commit_pair(&empty[s]);
+          mma_commit_pair(&d_full[buf]);
+          if (++s == kBigStages) {
+            s = 0;
+            ph ^= 1;
+          }
+        }
+      if (*abort_flag) {  // the MMAs in flight end before the tensor memory is freed
+        mma_commit_pair(drained);
+        mbar_wait_bounded(drained, 0, p.err, AH_ETIMEOUT, kWaitLimit);
+      }
+    }
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kBigRegsMany));
+    const int q = warp & 3, h = (warp - 4) >> 2;  // TMEM lane quarter, column half
+    const uint32_t d_empty0 = mapa_shared(smem_u32(d_empty), 0);
+    const uint32_t lane_addr = tmem + ((uint32_t)(q * 32) << 16) + h * 64;
+    const bool vec = (reinterpret_cast<uintptr_t>(g.ascales) & 15) == 0 && g.lds % 4 == 0;
+    const bool wvec = kb % 4 == 0;
+    uint8_t* stage = smem + Big::kStage + (warp - 4) * 4096;
+    pdl_wait();  // the scales come from the preceding grid
+    int n = 0;
+    bool ok = true;
+    for (int tile = first; tile < tiles; tile += step) {
+      const int unit = tile / mt, m0 = tile % mt * kBigTokens + rank * 128 + q * 32;
+      const int64_t tok = m0 + lane;
+      const float* arow = g.ascales + (tok < g.m ? tok : 0) * g.lds;  // past m: stored nowhere
+      const float* w0 = g.wscales + (int64_t)(unit * 2) * kb;
+      const float* w1 = g.wscales + (int64_t)min(unit * 2 + 1, nt - 1) * kb;
+      float acc[2][64];
+#pragma unroll
+      for (int j = 0; j < 64; ++j) acc[0][j] = acc[1][j] = 0.0f;
+      float a4[4];
+      load_scales4(arow, 0, kb, vec, a4);
+      for (int b4 = 0; b4 < kb; b4 += 4) {
+        float s0[4], s1[4];
+        load_scales4(w0, b4, kb, wvec, s0);
+        load_scales4(w1, b4, kb, wvec, s1);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          s0[i] *= a4[i];
+          s1[i] *= a4[i];
+        }
+        load_scales4(arow, b4 + 4, kb, vec, a4);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          if (b4 + i >= kb) break;
+          const int buf = (int)(n & 1);
+          if (lane == 0) ok = !*abort_flag && wait_or_abort(&d_full[buf], (uint32_t)((n / 2) & 1), p.err, abort_flag);
+          ok = __shfl_sync(0xFFFFFFFFu, ok, 0);
+          ++n;
+          if (!ok) continue;
+          tc_fence_after();
+          const uint32_t ta = lane_addr + buf * 256;
+          uint32_t v[2][32];
+          tmem_ld32_issue(ta, v[0]);
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            tmem_ld32_wait(v[c & 1]);
+            if (c < 3) {
+              tmem_ld32_issue(ta + (c + 1) / 2 * 128 + (c + 1) % 2 * 32, v[(c + 1) & 1]);
+            } else {
+              tc_fence_before();
+              __syncwarp();
+              if (lane == 0) mbar_arrive_cluster(d_empty0 + buf * 8);
+            }
+            const float f = c < 2 ? s0[i] : s1[i];
+#pragma unroll
+            for (int j = 0; j < 32; ++j) {
+              float& o = acc[c / 2][c % 2 * 32 + j];
+              o = fmaf(__uint_as_float(v[c & 1][j]), f, o);
+            }
+          }
+        }
+      }
+      // after a give-up the warps still meet at the barriers below
+      if constexpr (kGlu) {
+        const int64_t n_ff = g.rows / 2, c0 = (int64_t)unit * kFp8Group + h * 64;
+        uint32_t mx = __float_as_uint(kFp8Tiny);
+#pragma unroll
+        for (int j = 0; j < 64; ++j) {
+          // rows past n_ff are zero in the images: their products are zero
+          acc[0][j] = fp8_silu_mul_fast(acc[0][j], acc[1][j]);
+          mx = max(mx, __float_as_uint(acc[0][j]) & 0x7FFFFFFFu);
+        }
+        uint32_t* maxima = reinterpret_cast<uint32_t*>(smem + Big::kMax);
+        maxima[h * 128 + q * 32 + lane] = mx;
+        asm volatile("bar.sync 1, 256;" ::: "memory");
+        mx = max(mx, maxima[(h ^ 1) * 128 + q * 32 + lane]);
+        asm volatile("bar.sync 1, 256;" ::: "memory");  // read before the next tile writes
+        const float gm = __uint_as_float(mx), inv = __fdiv_rn(kFp8Max, gm);
+        if (ok && tok < g.m) {
+          uint8_t* qrow = p.act_q + tok * p.ld_act + c0;  // 16-byte aligned: ld_act is a multiple of 16
+#pragma unroll
+          for (int j = 0; j < 64; j += 16) {
+            uint32_t w[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+              w[i] = cvt_e4m3x4(acc[0][j + 4 * i] * inv, acc[0][j + 4 * i + 1] * inv, acc[0][j + 4 * i + 2] * inv,
+                                acc[0][j + 4 * i + 3] * inv);
+            if (c0 + j + 16 <= n_ff) {
+              *reinterpret_cast<uint4*>(qrow + j) = make_uint4(w[0], w[1], w[2], w[3]);
+            } else {
+#pragma unroll
+              for (int i = 0; i < 16; ++i)
+                if (c0 + j + i < n_ff) qrow[j + i] = (uint8_t)(w[i / 4] >> (8 * (i % 4)));
+            }
+          }
+          if (h == 0) p.act_scales[tok * p.lds_act + unit] = gm * (1.0f / kFp8Max);
+        }
+      } else if (!ok) {
+        continue;
+      } else if (p.y_map) {
+        // 128-byte rows through the warp's 4 KB stage (16-byte pieces swizzled as
+        // the map does), one tiled store per 32 rows
+        const bool wide = g.y_dtype == AH_DTYPE_F32;
+        const uint32_t row = smem_u32(stage) + lane * 128, sw = lane & 7;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) {
+          if (!wide && (c & 1)) continue;
+          const int64_t col = (int64_t)(unit * 2 + c / 2) * kFp8Group + h * 64 + c % 2 * 32;
+          if (lane == 0) bulk_wait_read0();  // the last store has read the stage
+          __syncwarp();
+#pragma unroll
+          for (int j = 0; j < 8; ++j) {
+            uint32_t w[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+              const float* o = &acc[c / 2][0];
+              if (wide) w[i] = __float_as_uint(o[c % 2 * 32 + 4 * j + i]);
+              else if (c % 2 == 0) {
+                const int k = (8 * j + 2 * i) & 63;
+                w[i] = g.y_dtype == AH_DTYPE_F16 ? pack2<__half>(o[k], o[k + 1]) : pack2<__nv_bfloat16>(o[k], o[k + 1]);
+              }
+            }
+            asm volatile("st.shared.v4.b32 [%0], {%1, %2, %3, %4};" ::"r"(row + ((j ^ sw) << 4)), "r"(w[0]), "r"(w[1]),
+                         "r"(w[2]), "r"(w[3])
+                         : "memory");
+          }
+          fence_proxy_async_smem();
+          __syncwarp();
+          if (lane == 0 && col < g.rows && m0 < g.m) {
+            tma_store_2d(&p.tm_y, (int)col, (int)m0, smem_u32(stage));
+            bulk_commit();
+          }
+        }
+      } else if (tok < g.m) {
+        const int64_t rows = g.gate_up ? g.rows / 2 : g.rows;  // rows of a tile's source
+#pragma unroll
+        for (int c = 0; c < 2; ++c) {
+          const int64_t r0 = (int64_t)(g.gate_up ? unit : unit * 2 + c) * kFp8Group + h * 64;
+          const int64_t base = tok * g.ldy + (g.gate_up ? c * rows : 0) + r0;
+#pragma unroll
+          for (int j = 0; j < 64; ++j)
+            if (r0 + j < rows) store_y(g.y, base + j, g.y_dtype, acc[c][j]);
+        }
+      }
+    }
+    if (lane == 0) bulk_wait_all();  // the stage is read, the stores complete
+  }
+
+  __syncwarp();
+  __syncthreads();
+  cluster_arrive();
+  cluster_wait();
+  if (warp == 1) {
+    tc_fence_after();
+    tmem_dealloc_pair(tmem, 512);
+  }
+}
+
+template <bool kGlu>
+int launch_big(BigArgs& p, cudaStream_t st) {
+  const MatmulArgs& g = p.g;
+  int rc = encode_rows(&p.tm_a, g.a, (uint64_t)g.cols, (uint64_t)g.m, (uint64_t)g.lda, 128);
+  if (rc != AH_OK) return rc;
+  rc = encode_2d(&p.tm_w, g.tiles, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, kFp8Group, (uint64_t)g.nt * g.kb * kFp8Group,
+                 kFp8Group, kFp8Group, CU_TENSOR_MAP_SWIZZLE_NONE);
+  if (rc != AH_OK) return rc;
+  const int elem = g.y_dtype == AH_DTYPE_F32 ? 4 : 2;
+  p.y_map = !kGlu && !g.gate_up && aligned16(g.y) && g.ldy * elem % 16 == 0;
+  if (p.y_map) {
+    const CUtensorMapDataType dt = elem == 4 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_UINT16;
+    auto fn = tensor_map_encoder();
+    const cuuint64_t dims[2] = {(cuuint64_t)g.rows, (cuuint64_t)g.m}, strides[1] = {(cuuint64_t)g.ldy * elem};
+    const cuuint32_t box[2] = {(cuuint32_t)(128 / elem), 32}, one[2] = {1, 1};
+    const CUresult r = fn(&p.tm_y, dt, 2, g.y, dims, strides, box, one, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                          CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_NONE,
+                          CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return fail(AH_ECUDA, "fp8w_matmul: cuTensorMapEncodeTiled failed (%d)", (int)r);
+  }
+  static std::once_flag once[64];
+  static cudaError_t attr[64];
+  int dev = 0;
+  rc = device_once(&dev);
+  if (rc != AH_OK) return rc;
+  std::call_once(once[dev], [&] {
+    attr[dev] = cudaFuncSetAttribute(k_fp8_big<kGlu>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Big::kDynamic);
+  });
+  AH_CUDA_TRY(attr[dev]);
+  const int64_t tiles = (g.m + kBigTokens - 1) / kBigTokens * ((g.nt + 1) / 2);
+  AH_REQUIRE(tiles < (1 << 30) && g.nt * g.kb < (1 << 24) && g.m <= 0x7FFFFF00,
+             "fp8w_matmul: too many tiles for one launch");
+  const int64_t pairs = std::min<int64_t>(tiles, sm_count() / 2);
+  return launch_pdl(k_fp8_big<kGlu>, dim3((unsigned)(2 * pairs)), dim3(kBigThreads), Big::kDynamic, st,
+                    (const BigArgs)p);
+}
+
+bool use_big(int64_t m) { return m > 128; }
+
 int check_device(const char* who, const AhFp8Weight* w) {
   int dev = -1;
   AH_CUDA_TRY(cudaGetDevice(&dev));
@@ -598,6 +981,12 @@ int matmul(const AhFp8Weight* w, const uint8_t* q, int64_t ldq, const float* sca
   if (rc != AH_OK) return rc;
   const MatmulArgs g{w->tiles, w->scales, w->rows, w->cols, w->nt, w->kb, w->gate_up, q, ldq, scales, lds, m, y, ldy,
                      y_dtype};
+  if (use_big(m)) {
+    BigArgs p{};
+    p.g = g;
+    p.err = device_error_word();
+    return launch_big<false>(p, st);
+  }
   SmallArgs p{};
   p.g = g;
   p.err = device_error_word();
@@ -607,14 +996,16 @@ int matmul(const AhFp8Weight* w, const uint8_t* q, int64_t ldq, const float* sca
 // silu(gate) * up of the products with a gate/up weight, quantised from f32.
 int matmul_swiglu(const AhFp8Weight* w, const uint8_t* q, int64_t ldq, const float* scales, int64_t lds, int64_t m,
                   uint8_t* act_q, int64_t ld_act, float* act_scales, int64_t lds_act, cudaStream_t st) {
-  SmallArgs p{};
-  p.g = MatmulArgs{w->tiles, w->scales, w->rows, w->cols, w->nt, w->kb, true, q, ldq, scales, lds, m, nullptr, 0, 0};
-  p.act_q = act_q;
-  p.ld_act = ld_act;
-  p.act_scales = act_scales;
-  p.lds_act = lds_act;
-  p.err = device_error_word();
-  return dispatch_small<true>(p, st);
+  auto run = [&](auto p, auto launch) {
+    p.g = MatmulArgs{w->tiles, w->scales, w->rows, w->cols, w->nt, w->kb, true, q, ldq, scales, lds, m, nullptr, 0, 0};
+    p.act_q = act_q;
+    p.ld_act = ld_act;
+    p.act_scales = act_scales;
+    p.lds_act = lds_act;
+    p.err = device_error_word();
+    return launch(p, st);
+  };
+  return use_big(m) ? run(BigArgs{}, launch_big<true>) : run(SmallArgs{}, dispatch_small<true>);
 }
 
 // ---- the feed-forward block ----------------------------------------------------------
