@@ -278,11 +278,18 @@ struct SmallArgs {
   int* err;
 };
 
-// Waits on `bar`'s phase `parity`; on give-up raises the CTA's abort flag.
-__device__ __forceinline__ bool wait_or_abort(uint64_t* bar, uint32_t parity, int* err, volatile int* abort_flag) {
-  if (mbar_wait_bounded(bar, parity, err, AH_ETIMEOUT, kWaitLimit)) return true;
+// Waits on `bar`'s phase `parity`, up to kWaitLimit polls; then records
+// AH_ETIMEOUT, raises the CTA's abort flag and goes on, as every later wait of
+// the CTA then does at once: the outputs are lost, but all copies and MMAs stay
+// inside the CTA's own stages and buffers and the kernel ends.
+__device__ __forceinline__ void wait_bar(uint64_t* bar, uint32_t parity, int* err, volatile int* abort_flag) {
+  if (mbar_try_wait(bar, parity)) return;
+  for (uint32_t it = 0; it < kWaitLimit; ++it) {
+    if (mbar_try_wait(bar, parity)) return;
+    if ((it & 63) == 0 && *abort_flag) return;
+  }
   *abort_flag = 1;
-  return false;
+  if (err) atomicExch(err, AH_ETIMEOUT);
 }
 
 __device__ __forceinline__ void promote_barrier() { asm volatile("bar.sync 1, 128;" ::: "memory"); }
@@ -301,7 +308,7 @@ __global__ void __launch_bounds__(kSmallThreads, 2) k_fp8_small(const __grid_con
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + L::kMisc + 4);
   const MatmulArgs& g = p.g;
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int warp = warp_index(), lane = threadIdx.x & 31;
   const int nc = (int)gridDim.x, rank = (int)blockIdx.x;  // the cluster spans x
   const int64_t unit = blockIdx.y;                        // tile, or gate/up pair
   const int64_t m0 = (int64_t)blockIdx.z * kNt;
@@ -332,57 +339,63 @@ __global__ void __launch_bounds__(kSmallThreads, 2) k_fp8_small(const __grid_con
   const uint32_t tmem = *tmem_slot;
 
   if (warp == 0) {
-    if (lane == 0) {
-      const uint8_t* src = g.tiles + fp8_image(g.gate_up, g.kb, unit * L::kTiles, b0) * kFp8TileBytes;
-      const bool halves = !kGlu && g.gate_up;  // one of a pair's two images per column block
-      auto blocks = [&](int s) { return min(L::kKs, nb - s * L::kKs); };
-      auto weights = [&](int s) {
-        const int r = s % L::kStages, n = blocks(s);
-        mbar_arrive_expect_tx(&full[r], (uint32_t)(n * (L::kBlockBytes + L::kActBytes)));
-        uint8_t* dst = smem + r * L::kStageBytes;
-        if (!halves)
-          bulk_g2s(dst, src + (size_t)s * L::kKs * L::kBlockBytes, (uint32_t)(n * L::kBlockBytes), &full[r]);
-        else
-          for (int i = 0; i < n; ++i)
-            bulk_g2s(dst + i * kFp8TileBytes, src + (size_t)(s * L::kKs + i) * 2 * kFp8TileBytes, kFp8TileBytes,
-                     &full[r]);
-      };
-      auto tokens = [&](int s) {
-        const int r = s % L::kStages;
-        uint8_t* dst = smem + r * L::kStageBytes + L::kKs * L::kBlockBytes;
-        for (int i = 0; i < blocks(s); ++i)
-          tma_load_2d(dst + i * L::kActBytes, &p.tm_a, (int)(b0 + s * L::kKs + i) * kFp8Group, (int)m0, &full[r]);
-      };
-      const int ahead = min(n_stage, L::kStages);
-      for (int s = 0; s < ahead; ++s) weights(s);
-      pdl_wait();  // the tokens come from the preceding grid
-      for (int s = 0; s < ahead; ++s) tokens(s);
-      int issued = ahead;
-      for (int s = ahead; s < n_stage; ++s) {
-        if (*abort_flag ||
-            !wait_or_abort(&empty[s % L::kStages], (uint32_t)((s / L::kStages - 1) & 1), p.err, abort_flag))
-          break;
-        weights(s);
-        tokens(s);
-        ++issued;
+    const bool elected = elect_one();
+    const uint8_t* src = g.tiles + fp8_image(g.gate_up, g.kb, unit * L::kTiles, b0) * kFp8TileBytes;
+    const bool halves = !kGlu && g.gate_up;  // one of a pair's two images per column block
+    auto weights = [&](int s, int r) {
+      const int n = min(L::kKs, nb - s * L::kKs);
+      uint8_t* dst = smem + r * L::kStageBytes;
+      mbar_arrive_expect_tx(&full[r], (uint32_t)(n * (L::kBlockBytes + L::kActBytes)));
+      if (!halves)
+        bulk_g2s(dst, src + (int64_t)s * L::kKs * L::kBlockBytes, (uint32_t)(n * L::kBlockBytes), &full[r]);
+      else
+        for (int i = 0; i < n; ++i)
+          bulk_g2s(dst + i * kFp8TileBytes, src + (int64_t)(s * L::kKs + i) * 2 * kFp8TileBytes, kFp8TileBytes,
+                   &full[r]);
+    };
+    const int x0 = (int)b0 * kFp8Group;
+    auto tokens = [&](int s, int r) {
+      const int n = min(L::kKs, nb - s * L::kKs);
+      uint8_t* dst = smem + r * L::kStageBytes + L::kKs * L::kBlockBytes;
+      for (int i = 0; i < n; ++i)
+        tma_load_2d(dst + i * L::kActBytes, &p.tm_a, x0 + (s * L::kKs + i) * kFp8Group, (int)m0, &full[r]);
+    };
+    const int ahead = min(n_stage, L::kStages);
+    if (elected)
+      for (int s = 0; s < ahead; ++s) weights(s, s);
+    pdl_wait();  // the tokens come from the preceding grid
+    if (elected)
+      for (int s = 0; s < ahead; ++s) tokens(s, s);
+    int r = 0;
+    uint32_t ph = 0;
+    for (int s = ahead; s < n_stage; ++s) {
+      wait_bar(&empty[r], ph, p.err, abort_flag);
+      if (elected) {
+        weights(s, r);
+        tokens(s, r);
       }
-      if (*abort_flag)  // the copies in flight land before the CTA can exit
-        for (int s = max(0, issued - L::kStages); s < issued; ++s)
-          mbar_wait_bounded(&full[s % L::kStages], (uint32_t)((s / L::kStages) & 1), p.err, AH_ETIMEOUT, kWaitLimit);
+      if (++r == L::kStages) {
+        r = 0;
+        ph ^= 1;
+      }
     }
+    if (*abort_flag)  // the copies in flight land before the CTA can exit
+      for (int s = max(0, n_stage - L::kStages); s < n_stage; ++s)
+        mbar_wait_bounded(&full[s % L::kStages], (uint32_t)((s / L::kStages) & 1), p.err, AH_ETIMEOUT, 1u << 12);
   } else if (warp == 1) {
-    if (lane == 0) {
-      constexpr uint32_t idesc = idesc_e4m3(128, kNt);
-      for (int i = 0; i < nb; ++i) {
-        const int s = i / L::kKs, r = s % L::kStages, buf = i % L::kBufs;
-        if (*abort_flag) break;
-        if (i % L::kKs == 0 && !wait_or_abort(&full[r], (uint32_t)((s / L::kStages) & 1), p.err, abort_flag)) break;
-        if (i >= L::kBufs && !wait_or_abort(&d_empty[buf], (uint32_t)((i / L::kBufs - 1) & 1), p.err, abort_flag))
-          break;
-        tc_fence_after();
-        const uint32_t st = smem_u32(smem + r * L::kStageBytes);
-        const uint32_t wb = st + (i % L::kKs) * L::kBlockBytes;
-        const uint64_t bdesc = sw128_desc(st + L::kKs * L::kBlockBytes + (i % L::kKs) * L::kActBytes);
+    const bool elected = elect_one();
+    constexpr uint32_t idesc = idesc_e4m3(128, kNt);
+    int r = 0, buf = 0;
+    uint32_t ph = 0, dph = 1;  // the buffers start empty
+    for (int i = 0; i < nb; ++i) {
+      if (i % L::kKs == 0) wait_bar(&full[r], ph, p.err, abort_flag);
+      wait_bar(&d_empty[buf], dph, p.err, abort_flag);
+      tc_fence_after();
+      const uint32_t st = smem_u32(smem + r * L::kStageBytes);
+      const uint32_t wb = st + (i % L::kKs) * L::kBlockBytes;
+      const uint64_t bdesc = sw128_desc(st + L::kKs * L::kBlockBytes + (i % L::kKs) * L::kActBytes);
+      const bool last = i % L::kKs == L::kKs - 1 || i == nb - 1;
+      if (elected) {
 #pragma unroll
         for (int h = 0; h < L::kTiles; ++h) {
           const uint64_t adesc = sw128_desc(wb + h * kFp8TileBytes);
@@ -390,13 +403,21 @@ __global__ void __launch_bounds__(kSmallThreads, 2) k_fp8_small(const __grid_con
           for (int kk = 0; kk < 4; ++kk)
             mma_f8(tmem + buf * L::kCols + h * kNt, adesc + kk * 2, bdesc + kk * 2, idesc, kk > 0);
         }
-        if (i % L::kKs == L::kKs - 1 || i == nb - 1) mma_commit(&empty[r]);
         mma_commit(&d_full[buf]);
+        if (last) mma_commit(&empty[r]);
       }
-      if (*abort_flag) {  // the MMAs in flight end before the tensor memory is freed
-        mma_commit(drained);
-        mbar_wait_bounded(drained, 0, p.err, AH_ETIMEOUT, kWaitLimit);
+      if (last && ++r == L::kStages) {
+        r = 0;
+        ph ^= 1;
       }
+      if (++buf == L::kBufs) {
+        buf = 0;
+        dph ^= 1;
+      }
+    }
+    if (*abort_flag) {  // the MMAs in flight end before the tensor memory is freed
+      if (elected) mma_commit(drained);
+      mbar_wait_bounded(drained, 0, p.err, AH_ETIMEOUT, kWaitLimit);
     }
   } else {
     const int q = warp & 3, t = threadIdx.x - 64;  // TMEM lane quarter, reader index
@@ -420,9 +441,9 @@ __global__ void __launch_bounds__(kSmallThreads, 2) k_fp8_small(const __grid_con
     float acc[L::kCols];
 #pragma unroll
     for (int j = 0; j < L::kCols; ++j) acc[j] = 0.0f;
-    bool ok = true;
+    int buf = 0;
+    uint32_t ph = 0;
     for (int i = 0; i < nb; ++i) {
-      const int buf = i % L::kBufs;
       float* set = sc + (i / kScaleBlocks & 1) * kScaleBlocks * L::kCols;
       if (i % kScaleBlocks == 0) {
 #pragma unroll
@@ -434,31 +455,31 @@ __global__ void __launch_bounds__(kSmallThreads, 2) k_fp8_small(const __grid_con
         promote_barrier();
         fetch(i + kScaleBlocks);
       }
-      if (lane == 0)
-        ok = !*abort_flag && wait_or_abort(&d_full[buf], (uint32_t)((i / L::kBufs) & 1), p.err, abort_flag);
-      ok = __shfl_sync(0xFFFFFFFFu, ok, 0);
-      if (ok) {
-        tc_fence_after();
-        const float* s = set + i % kScaleBlocks * L::kCols;
-        const uint32_t ta = tmem + ((uint32_t)(q * 32) << 16) + buf * L::kCols;
-        constexpr int kStep = L::kCols < 32 ? 16 : 32;
+      wait_bar(&d_full[buf], ph, p.err, abort_flag);
+      tc_fence_after();
+      const float* s = set + i % kScaleBlocks * L::kCols;
+      const uint32_t ta = tmem + ((uint32_t)(q * 32) << 16) + buf * L::kCols;
+      constexpr int kStep = L::kCols < 32 ? 16 : 32;
 #pragma unroll
-        for (int c = 0; c < L::kCols; c += kStep) {
-          float v[kStep];
-          if constexpr (kStep == 16) tmem_ld16(ta + c, v);
-          else tmem_ld32(ta + c, v);
+      for (int c = 0; c < L::kCols; c += kStep) {
+        float v[kStep];
+        if constexpr (kStep == 16) tmem_ld16(ta + c, v);
+        else tmem_ld32(ta + c, v);
 #pragma unroll
-          for (int j = 0; j < kStep; j += 4) {
-            const float4 f = *reinterpret_cast<const float4*>(s + c + j);
-            acc[c + j] = fmaf(v[j], f.x, acc[c + j]);
-            acc[c + j + 1] = fmaf(v[j + 1], f.y, acc[c + j + 1]);
-            acc[c + j + 2] = fmaf(v[j + 2], f.z, acc[c + j + 2]);
-            acc[c + j + 3] = fmaf(v[j + 3], f.w, acc[c + j + 3]);
-          }
+        for (int j = 0; j < kStep; j += 4) {
+          const float4 f = *reinterpret_cast<const float4*>(s + c + j);
+          acc[c + j] = fmaf(v[j], f.x, acc[c + j]);
+          acc[c + j + 1] = fmaf(v[j + 1], f.y, acc[c + j + 1]);
+          acc[c + j + 2] = fmaf(v[j + 2], f.z, acc[c + j + 2]);
+          acc[c + j + 3] = fmaf(v[j + 3], f.w, acc[c + j + 3]);
         }
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(&d_empty[buf]);
+      }
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(&d_empty[buf]);
+      if (++buf == L::kBufs) {
+        buf = 0;
+        ph ^= 1;
       }
     }
     // every block's MMAs have read their stages: the ring is idle
@@ -583,34 +604,29 @@ int dispatch_small(SmallArgs& p, cudaStream_t st) {
   if constexpr (!kGlu) return launch_small<128, false>(p, st);
 }
 
-// ---- many tokens: CTA pairs, 256 tokens x 256 weight rows ---------------------------------
+// ---- many tokens: 128 tokens x 256 weight rows per CTA -------------------------------------
 //
-// A persistent pair walks tiles of 256 tokens x two weight tiles (a gate/up pair
-// for SwiGLU).  Each CTA loads its 128 tokens and one of the two weight images of
-// a column block (32 KB) and holds all 256 columns of its tokens' sums:
+// A persistent CTA walks tiles of 128 tokens x two weight tiles (a gate/up pair
+// for SwiGLU):
 //
-//   warp 0     producer (both CTAs, all copies complete on the leader's barrier)
-//   warp 1     TMEM owner; in the leader the MMA issuer: cta_group::2, M = 256,
-//              N = 256, K = 32, four per column block into one of two buffers of
-//              256 tensor-memory columns
+//   warp 0     producer: a TMA box of the tokens and the two weight images of a
+//              column block per stage (48 KB)
+//   warp 1     TMEM owner, MMA issuer: M = 128, N = 256, K = 32, four per column
+//              block into one of two buffers of 256 tensor-memory columns
 //   warps 4-11 a thread owns one token (tensor-memory lane) and 64 columns of each
 //              weight tile: sums times a_scale * w_scale into 128 f32 registers,
 //              one multiply-add each, since w_scale is one number per weight tile
 //              and column block; then the tile's output
-//
-// Both CTAs read half of B from each other's shared memory, so a pair moves
-// 64 KB per column block for 512 x 128 operand columns where two single CTAs of
-// 128 x 256 would move 96 KB.
 
-constexpr int kBigStages = 6;
+constexpr int kBigStages = 4;
 constexpr int kBigThreads = 384;
 // Registers: 384 threads start with 168 each (64512); the first four warps drop
 // to 40 and the eight readers rise to 232 (128 * 40 + 256 * 232 = 64512).
 constexpr int kBigRegsFew = 40, kBigRegsMany = 232;
-constexpr int kBigTokens = 256;
+constexpr int kBigTokens = 128;
 
 struct Big {
-  static constexpr int kStageBytes = 2 * kFp8TileBytes;  // 128 tokens, one weight image
+  static constexpr int kStageBytes = 3 * kFp8TileBytes;    // 128 tokens, two weight images
   static constexpr int kStage = kBigStages * kStageBytes;  // output staging: 4 KB per reader warp
   static constexpr int kMax = kStage + 8 * 4096;           // SwiGLU: group maxima [2][128]
   static constexpr int kBars = kMax + 1024;
@@ -622,7 +638,6 @@ struct Big {
 
 struct BigArgs {
   CUtensorMap tm_a;  // e4m3 activations [m][cols], box 128 x 128, 128-byte swizzle
-  CUtensorMap tm_w;  // weight images as bytes [images * 128][128], box 128 x 128
   CUtensorMap tm_y;  // y [m][rows], box 128 bytes x 32 rows, 128-byte swizzle (when y_map)
   MatmulArgs g;
   bool y_map;
@@ -662,22 +677,21 @@ __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float a, float b) {
 }
 
 template <bool kGlu>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kBigThreads, 1) k_fp8_big(const __grid_constant__ BigArgs p) {
+__global__ void __launch_bounds__(kBigThreads, 1) k_fp8_big(const __grid_constant__ BigArgs p) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint64_t* full = reinterpret_cast<uint64_t*>(smem + Big::kBars);  // the leader's are used
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + Big::kBars);
   uint64_t* empty = full + kBigStages;
   uint64_t* d_full = empty + kBigStages;
-  uint64_t* d_empty = d_full + 2;  // the leader's are used
+  uint64_t* d_empty = d_full + 2;
   uint64_t* drained = d_empty + 2;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + Big::kMisc);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + Big::kMisc + 4);
   const MatmulArgs& g = p.g;
 
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int rank = (int)cluster_ctarank();
+  const int warp = warp_index(), lane = threadIdx.x & 31;
   const int mt = (int)((g.m + kBigTokens - 1) / kBigTokens), nt = (int)g.nt, kb = (int)g.kb;
-  const int tiles = mt * ((nt + 1) / 2), first = blockIdx.x / 2, step = gridDim.x / 2;
+  const int tiles = mt * ((nt + 1) / 2), first = blockIdx.x, step = gridDim.x;
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < kBigStages; ++i) {
@@ -686,94 +700,102 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kBigThreads, 1) k_fp
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&d_full[i], 1);
-      mbar_init(&d_empty[i], 16);  // eight reader warps in each CTA
+      mbar_init(&d_empty[i], 8);  // the reader warps
     }
     mbar_init(drained, 1);
     *abort_flag = 0;
     fence_mbar_init();
   }
-  if (warp == 1) tmem_alloc_pair(tmem_slot, 512);
+  if (warp == 1) tmem_alloc(tmem_slot, 512);
   tc_fence_before();
   __syncthreads();
-  cluster_arrive();
-  cluster_wait();
   tc_fence_after();
   pdl_launch_dependents();  // after the allocation, as in k_fp8_small
   const uint32_t tmem = *tmem_slot;
 
   if (warp < 4) {
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kBigRegsFew));
-    if (threadIdx.x == 0) {
-      // a stage's copies land in both CTAs and complete on the leader's barrier
-      const uint32_t full0 = mapa_shared(smem_u32(full), 0), st0 = smem_u32(smem);
-      auto weights = [&](int s, int tile, int b) {
-        if (rank == 0) mbar_arrive_expect_tx(&full[s], 2 * Big::kStageBytes);
-        const int t = min(tile / mt * 2 + rank, nt - 1);  // past an odd last tile: read again, not stored
-        tma_load_2d_pair(st0 + s * Big::kStageBytes + kFp8TileBytes, &p.tm_w, 0,
-                         (int)fp8_image(g.gate_up, kb, t, b) * kFp8Group, full0 + s * 8);
-      };
-      const int ahead = min(kb, kBigStages);
-      for (int i = 0; i < ahead; ++i) weights(i, first, i);
-      pdl_wait();  // the tokens come from the preceding grid
-      int s = 0, left = ahead, round = 0;  // stage, blocks whose weights are under way, passes over the ring
-      for (int tile = first; tile < tiles && !*abort_flag; tile += step) {
-        const int row = tile % mt * kBigTokens + rank * 128;
-        for (int b = 0; b < kb; ++b) {
-          if (round > 0 &&
-              (*abort_flag || !wait_or_abort(&empty[s], (uint32_t)((round - 1) & 1), p.err, abort_flag)))
-            break;
-          if (left > 0) --left;
-          else weights(s, tile, b);
-          tma_load_2d_pair(st0 + s * Big::kStageBytes, &p.tm_a, b * kFp8Group, row, full0 + s * 8);
-          if (++s == kBigStages) {
-            s = 0;
-            ++round;
-          }
+    if (warp == 0) {
+      const bool elected = elect_one();
+      auto weights = [&](int s, int unit, int b) {
+        uint8_t* dst = smem + s * Big::kStageBytes + kFp8TileBytes;
+        mbar_arrive_expect_tx(&full[s], Big::kStageBytes);
+        const uint8_t* w0 = g.tiles + fp8_image(g.gate_up, kb, unit * 2, b) * kFp8TileBytes;
+        if (g.gate_up) {
+          bulk_g2s(dst, w0, 2 * kFp8TileBytes, &full[s]);
+        } else {
+          // past an odd last tile the first is read again, and not stored
+          bulk_g2s(dst, w0, kFp8TileBytes, &full[s]);
+          bulk_g2s(dst + kFp8TileBytes, unit * 2 + 1 < nt ? w0 + (int64_t)kb * kFp8TileBytes : w0, kFp8TileBytes,
+                   &full[s]);
         }
-      }
-      if (*abort_flag && rank == 0)  // the copies in flight land before the pair can exit
-        for (int i = 0; i < kBigStages; ++i)
-          if (i < s || round > 0)
-            mbar_wait_bounded(&full[i], (uint32_t)((i < s ? round : round - 1) & 1), p.err, AH_ETIMEOUT, kWaitLimit);
-    } else if (threadIdx.x == 32 && rank == 0) {
-      constexpr uint32_t idesc = idesc_e4m3(256, 256);
-      int s = 0, n = 0;
-      uint32_t ph = 0;
-      for (int tile = first; tile < tiles && !*abort_flag; tile += step)
-        for (int b = 0; b < kb; ++b, ++n) {
-          const int buf = n & 1;
-          if (*abort_flag || !wait_or_abort(&full[s], ph, p.err, abort_flag)) break;
-          if (n >= 2 && !wait_or_abort(&d_empty[buf], (uint32_t)((n / 2 - 1) & 1), p.err, abort_flag)) break;
-          tc_fence_after();
-          const uint32_t st = smem_u32(smem + s * Big::kStageBytes);
-          const uint64_t adesc = sw128_desc(st), bdesc = sw128_desc(st + kFp8TileBytes);
-#pragma unroll
-          for (int kk = 0; kk < 4; ++kk) mma_f8_pair(tmem + buf * 256, adesc + kk * 2, bdesc + kk * 2, idesc, kk > 0);
-          mma_commit_pair(&empty[s]);
-          mma_commit_pair(&d_full[buf]);
+      };
+      int left = min(kb, kBigStages);  // blocks whose weights are under way
+      if (elected)
+        for (int i = 0; i < left; ++i) weights(i, first / mt, i);
+      pdl_wait();  // the tokens come from the preceding grid
+      int s = 0;
+      uint32_t ph = 1;  // the stages start empty
+      for (int tile = first; tile < tiles; tile += step) {
+        const int unit = tile / mt, row = tile % mt * kBigTokens;
+        for (int b = 0; b < kb; ++b) {
+          wait_bar(&empty[s], ph, p.err, abort_flag);
+          if (elected) {
+            if (left <= 0) weights(s, unit, b);
+            tma_load_2d(smem + s * Big::kStageBytes, &p.tm_a, b * kFp8Group, row, &full[s]);
+          }
+          --left;
           if (++s == kBigStages) {
             s = 0;
             ph ^= 1;
           }
         }
+      }
+      if (*abort_flag)  // the copies in flight land before the CTA can exit
+        for (int i = 0; i < kBigStages; ++i)
+          mbar_wait_bounded(&full[i], i < s ? ph ^ 1 : ph, p.err, AH_ETIMEOUT, 1u << 12);
+    } else if (warp == 1) {
+      const bool elected = elect_one();
+      constexpr uint32_t idesc = idesc_e4m3(128, 256);
+      int s = 0, buf = 0;
+      uint32_t ph = 0, dph = 1;  // the buffers start empty
+      for (int tile = first; tile < tiles; tile += step)
+        for (int b = 0; b < kb; ++b) {
+          wait_bar(&full[s], ph, p.err, abort_flag);
+          wait_bar(&d_empty[buf], dph, p.err, abort_flag);
+          tc_fence_after();
+          const uint32_t st = smem_u32(smem + s * Big::kStageBytes);
+          const uint64_t adesc = sw128_desc(st), bdesc = sw128_desc(st + kFp8TileBytes);
+          if (elected) {
+#pragma unroll
+            for (int kk = 0; kk < 4; ++kk) mma_f8(tmem + buf * 256, adesc + kk * 2, bdesc + kk * 2, idesc, kk > 0);
+            mma_commit(&d_full[buf]);
+            mma_commit(&empty[s]);
+          }
+          if (++s == kBigStages) {
+            s = 0;
+            ph ^= 1;
+          }
+          buf ^= 1;
+          dph ^= buf == 0;
+        }
       if (*abort_flag) {  // the MMAs in flight end before the tensor memory is freed
-        mma_commit_pair(drained);
+        if (elected) mma_commit(drained);
         mbar_wait_bounded(drained, 0, p.err, AH_ETIMEOUT, kWaitLimit);
       }
     }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kBigRegsMany));
     const int q = warp & 3, h = (warp - 4) >> 2;  // TMEM lane quarter, column half
-    const uint32_t d_empty0 = mapa_shared(smem_u32(d_empty), 0);
     const uint32_t lane_addr = tmem + ((uint32_t)(q * 32) << 16) + h * 64;
     const bool vec = (reinterpret_cast<uintptr_t>(g.ascales) & 15) == 0 && g.lds % 4 == 0;
     const bool wvec = kb % 4 == 0;
     uint8_t* stage = smem + Big::kStage + (warp - 4) * 4096;
     pdl_wait();  // the scales come from the preceding grid
-    int n = 0;
-    bool ok = true;
+    int buf = 0;
+    uint32_t ph = 0;
     for (int tile = first; tile < tiles; tile += step) {
-      const int unit = tile / mt, m0 = tile % mt * kBigTokens + rank * 128 + q * 32;
+      const int unit = tile / mt, m0 = tile % mt * kBigTokens + q * 32;
       const int64_t tok = m0 + lane;
       const float* arow = g.ascales + (tok < g.m ? tok : 0) * g.lds;  // past m: stored nowhere
       const float* w0 = g.wscales + (int64_t)(unit * 2) * kb;
@@ -796,11 +818,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kBigThreads, 1) k_fp
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           if (b4 + i >= kb) break;
-          const int buf = (int)(n & 1);
-          if (lane == 0) ok = !*abort_flag && wait_or_abort(&d_full[buf], (uint32_t)((n / 2) & 1), p.err, abort_flag);
-          ok = __shfl_sync(0xFFFFFFFFu, ok, 0);
-          ++n;
-          if (!ok) continue;
+          wait_bar(&d_full[buf], ph, p.err, abort_flag);
           tc_fence_after();
           const uint32_t ta = lane_addr + buf * 256;
           uint32_t v[2][32];
@@ -813,7 +831,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kBigThreads, 1) k_fp
             } else {
               tc_fence_before();
               __syncwarp();
-              if (lane == 0) mbar_arrive_cluster(d_empty0 + buf * 8);
+              if (lane == 0) mbar_arrive(&d_empty[buf]);
             }
             const float f = c < 2 ? s0[i] : s1[i];
 #pragma unroll
@@ -822,9 +840,11 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kBigThreads, 1) k_fp
               o = fmaf(__uint_as_float(v[c & 1][j]), f, o);
             }
           }
+          buf ^= 1;
+          ph ^= buf == 0;
         }
       }
-      // after a give-up the warps still meet at the barriers below
+      const bool ok = !__any_sync(0xFFFFFFFFu, *abort_flag);  // after a give-up nothing is stored
       if constexpr (kGlu) {
         const int64_t n_ff = g.rows / 2, c0 = (int64_t)unit * kFp8Group + h * 64;
         uint32_t mx = __float_as_uint(kFp8Tiny);
@@ -912,11 +932,9 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kBigThreads, 1) k_fp
 
   __syncwarp();
   __syncthreads();
-  cluster_arrive();
-  cluster_wait();
   if (warp == 1) {
     tc_fence_after();
-    tmem_dealloc_pair(tmem, 512);
+    tmem_dealloc(tmem, 512);
   }
 }
 
@@ -924,9 +942,6 @@ template <bool kGlu>
 int launch_big(BigArgs& p, cudaStream_t st) {
   const MatmulArgs& g = p.g;
   int rc = encode_rows(&p.tm_a, g.a, (uint64_t)g.cols, (uint64_t)g.m, (uint64_t)g.lda, 128);
-  if (rc != AH_OK) return rc;
-  rc = encode_2d(&p.tm_w, g.tiles, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, kFp8Group, (uint64_t)g.nt * g.kb * kFp8Group,
-                 kFp8Group, kFp8Group, CU_TENSOR_MAP_SWIZZLE_NONE);
   if (rc != AH_OK) return rc;
   const int elem = g.y_dtype == AH_DTYPE_F32 ? 4 : 2;
   p.y_map = !kGlu && !g.gate_up && aligned16(g.y) && g.ldy * elem % 16 == 0;
@@ -952,9 +967,8 @@ int launch_big(BigArgs& p, cudaStream_t st) {
   const int64_t tiles = (g.m + kBigTokens - 1) / kBigTokens * ((g.nt + 1) / 2);
   AH_REQUIRE(tiles < (1 << 30) && g.nt * g.kb < (1 << 24) && g.m <= 0x7FFFFF00,
              "fp8w_matmul: too many tiles for one launch");
-  const int64_t pairs = std::min<int64_t>(tiles, sm_count() / 2);
-  return launch_pdl(k_fp8_big<kGlu>, dim3((unsigned)(2 * pairs)), dim3(kBigThreads), Big::kDynamic, st,
-                    (const BigArgs)p);
+  return launch_pdl(k_fp8_big<kGlu>, dim3((unsigned)std::min<int64_t>(tiles, sm_count())), dim3(kBigThreads),
+                    Big::kDynamic, st, (const BigArgs)p);
 }
 
 bool use_big(int64_t m) { return m > 128; }

@@ -79,6 +79,22 @@ __device__ __forceinline__ bool mbar_wait_bounded(uint64_t* bar, uint32_t parity
   return false;
 }
 
+// One lane of the converged warp.  Issuing bulk copies and MMAs under this
+// predicate in warp-uniform code keeps their operands in uniform registers; a
+// threadIdx.x test costs a register move per operand, ~200 cycles per copy.
+__device__ __forceinline__ bool elect_one() {
+  uint32_t r;
+  asm volatile(
+      "{\n\t.reg .pred p;\n\t"
+      "elect.sync _|p, 0xFFFFFFFF;\n\t"
+      "selp.u32 %0, 1, 0, p;\n\t}"
+      : "=r"(r));
+  return r != 0;
+}
+
+// This thread's warp index, known to be the same over the warp.
+__device__ __forceinline__ int warp_index() { return __shfl_sync(0xFFFFFFFFu, (int)(threadIdx.x >> 5), 0); }
+
 // Programmatic dependent launch: wait for the preceding grid's memory to be
 // visible / allow the next grid to start launching.
 __device__ __forceinline__ void pdl_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }

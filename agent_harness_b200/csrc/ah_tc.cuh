@@ -111,8 +111,11 @@ __device__ __forceinline__ void tma_load_2d_pair(uint32_t dst, const void* tmap,
       "l"(tmap), "r"(x), "r"(y), "r"(bar)
       : "memory");
 }
+// Arrives on another CTA's barrier.  What it orders here is tensor-memory reads,
+// which tcgen05.wait and tcgen05.fence have completed: a release at cluster scope
+// would add a memory barrier of several hundred cycles to every arrival.
 __device__ __forceinline__ void mbar_arrive_cluster(uint32_t bar) {
-  asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+  asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
 // A tiled store shared -> global (one bulk group per commit), clipped to the
 // map's extents.
