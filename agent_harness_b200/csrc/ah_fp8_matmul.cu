@@ -604,29 +604,30 @@ int dispatch_small(SmallArgs& p, cudaStream_t st) {
   if constexpr (!kGlu) return launch_small<128, false>(p, st);
 }
 
-// ---- many tokens: 128 tokens x 256 weight rows per CTA -------------------------------------
+// ---- many tokens: CTA pairs, 256 tokens x 256 weight rows ---------------------------------
 //
-// A persistent CTA walks tiles of 128 tokens x two weight tiles (a gate/up pair
-// for SwiGLU):
+// A persistent pair walks tiles of 256 tokens x two weight tiles (a gate/up pair
+// for SwiGLU).  Each CTA loads its 128 tokens and one of the two weight images of
+// a column block (32 KB) and holds all 256 columns of its tokens' sums:
 //
-//   warp 0     producer: a TMA box of the tokens and the two weight images of a
-//              column block per stage (48 KB)
-//   warp 1     TMEM owner, MMA issuer: M = 128, N = 256, K = 32, four per column
-//              block into one of two buffers of 256 tensor-memory columns
+//   warp 0     producer (both CTAs, all copies complete on the leader's barrier)
+//   warp 1     TMEM owner; in the leader the MMA issuer: cta_group::2, M = 256,
+//              N = 256, K = 32, four per column block into one of two buffers of
+//              256 tensor-memory columns
 //   warps 4-11 a thread owns one token (tensor-memory lane) and 64 columns of each
 //              weight tile: sums times a_scale * w_scale into 128 f32 registers,
 //              one multiply-add each, since w_scale is one number per weight tile
 //              and column block; then the tile's output
 
-constexpr int kBigStages = 4;
+constexpr int kBigStages = 6;
 constexpr int kBigThreads = 384;
 // Registers: 384 threads start with 168 each (64512); the first four warps drop
 // to 40 and the eight readers rise to 232 (128 * 40 + 256 * 232 = 64512).
 constexpr int kBigRegsFew = 40, kBigRegsMany = 232;
-constexpr int kBigTokens = 128;
+constexpr int kBigTokens = 256;
 
 struct Big {
-  static constexpr int kStageBytes = 3 * kFp8TileBytes;    // 128 tokens, two weight images
+  static constexpr int kStageBytes = 2 * kFp8TileBytes;    // 128 tokens, one weight image
   static constexpr int kStage = kBigStages * kStageBytes;  // output staging: 4 KB per reader warp
   static constexpr int kMax = kStage + 8 * 4096;           // SwiGLU: group maxima [2][128]
   static constexpr int kBars = kMax + 1024;
@@ -638,6 +639,7 @@ struct Big {
 
 struct BigArgs {
   CUtensorMap tm_a;  // e4m3 activations [m][cols], box 128 x 128, 128-byte swizzle
+  CUtensorMap tm_w;  // weight images as bytes [images * 128][128], box 128 x 128
   CUtensorMap tm_y;  // y [m][rows], box 128 bytes x 32 rows, 128-byte swizzle (when y_map)
   MatmulArgs g;
   bool y_map;
@@ -677,21 +679,22 @@ __device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float a, float b) {
 }
 
 template <bool kGlu>
-__global__ void __launch_bounds__(kBigThreads, 1) k_fp8_big(const __grid_constant__ BigArgs p) {
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kBigThreads, 1) k_fp8_big(const __grid_constant__ BigArgs p) {
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint64_t* full = reinterpret_cast<uint64_t*>(smem + Big::kBars);
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + Big::kBars);  // the leader's are used
   uint64_t* empty = full + kBigStages;
   uint64_t* d_full = empty + kBigStages;
-  uint64_t* d_empty = d_full + 2;
+  uint64_t* d_empty = d_full + 2;  // the leader's are used
   uint64_t* drained = d_empty + 2;
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + Big::kMisc);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + Big::kMisc + 4);
   const MatmulArgs& g = p.g;
 
   const int warp = warp_index(), lane = threadIdx.x & 31;
+  const int rank = (int)cluster_ctarank();
   const int mt = (int)((g.m + kBigTokens - 1) / kBigTokens), nt = (int)g.nt, kb = (int)g.kb;
-  const int tiles = mt * ((nt + 1) / 2), first = blockIdx.x, step = gridDim.x;
+  const int tiles = mt * ((nt + 1) / 2), first = blockIdx.x / 2, step = gridDim.x / 2;
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < kBigStages; ++i) {
@@ -700,15 +703,17 @@ __global__ void __launch_bounds__(kBigThreads, 1) k_fp8_big(const __grid_constan
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&d_full[i], 1);
-      mbar_init(&d_empty[i], 8);  // the reader warps
+      mbar_init(&d_empty[i], 16);  // eight reader warps in each CTA
     }
     mbar_init(drained, 1);
     *abort_flag = 0;
     fence_mbar_init();
   }
-  if (warp == 1) tmem_alloc(tmem_slot, 512);
+  if (warp == 1) tmem_alloc_pair(tmem_slot, 512);
   tc_fence_before();
   __syncthreads();
+  cluster_arrive();
+  cluster_wait();
   tc_fence_after();
   pdl_launch_dependents();  // after the allocation, as in k_fp8_small
   const uint32_t tmem = *tmem_slot;
@@ -717,18 +722,13 @@ __global__ void __launch_bounds__(kBigThreads, 1) k_fp8_big(const __grid_constan
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kBigRegsFew));
     if (warp == 0) {
       const bool elected = elect_one();
+      // a stage's copies land in both CTAs and complete on the leader's barrier
+      const uint32_t full0 = mapa_shared(smem_u32(full), 0), st0 = smem_u32(smem);
       auto weights = [&](int s, int unit, int b) {
-        uint8_t* dst = smem + s * Big::kStageBytes + kFp8TileBytes;
-        mbar_arrive_expect_tx(&full[s], Big::kStageBytes);
-        const uint8_t* w0 = g.tiles + fp8_image(g.gate_up, kb, unit * 2, b) * kFp8TileBytes;
-        if (g.gate_up) {
-          bulk_g2s(dst, w0, 2 * kFp8TileBytes, &full[s]);
-        } else {
-          // past an odd last tile the first is read again, and not stored
-          bulk_g2s(dst, w0, kFp8TileBytes, &full[s]);
-          bulk_g2s(dst + kFp8TileBytes, unit * 2 + 1 < nt ? w0 + (int64_t)kb * kFp8TileBytes : w0, kFp8TileBytes,
-                   &full[s]);
-        }
+        if (rank == 0) mbar_arrive_expect_tx(&full[s], 2 * Big::kStageBytes);
+        const int t = min(unit * 2 + rank, nt - 1);  // past an odd last tile: read again, not stored
+        tma_load_2d_pair(st0 + s * Big::kStageBytes + kFp8TileBytes, &p.tm_w, 0,
+                         (int)fp8_image(g.gate_up, kb, t, b) * kFp8Group, full0 + s * 8);
       };
       int left = min(kb, kBigStages);  // blocks whose weights are under way
       if (elected)
@@ -737,12 +737,12 @@ __global__ void __launch_bounds__(kBigThreads, 1) k_fp8_big(const __grid_constan
       int s = 0;
       uint32_t ph = 1;  // the stages start empty
       for (int tile = first; tile < tiles; tile += step) {
-        const int unit = tile / mt, row = tile % mt * kBigTokens;
+        const int unit = tile / mt, row = tile % mt * kBigTokens + rank * 128;
         for (int b = 0; b < kb; ++b) {
           wait_bar(&empty[s], ph, p.err, abort_flag);
           if (elected) {
             if (left <= 0) weights(s, unit, b);
-            tma_load_2d(smem + s * Big::kStageBytes, &p.tm_a, b * kFp8Group, row, &full[s]);
+            tma_load_2d_pair(st0 + s * Big::kStageBytes, &p.tm_a, b * kFp8Group, row, full0 + s * 8);
           }
           --left;
           if (++s == kBigStages) {
@@ -751,12 +751,12 @@ __global__ void __launch_bounds__(kBigThreads, 1) k_fp8_big(const __grid_constan
           }
         }
       }
-      if (*abort_flag)  // the copies in flight land before the CTA can exit
+      if (*abort_flag && rank == 0)  // the copies in flight land before the pair can exit
         for (int i = 0; i < kBigStages; ++i)
           mbar_wait_bounded(&full[i], i < s ? ph ^ 1 : ph, p.err, AH_ETIMEOUT, 1u << 12);
-    } else if (warp == 1) {
+    } else if (warp == 1 && rank == 0) {
       const bool elected = elect_one();
-      constexpr uint32_t idesc = idesc_e4m3(128, 256);
+      constexpr uint32_t idesc = idesc_e4m3(256, 256);
       int s = 0, buf = 0;
       uint32_t ph = 0, dph = 1;  // the buffers start empty
       for (int tile = first; tile < tiles; tile += step)
@@ -768,9 +768,9 @@ __global__ void __launch_bounds__(kBigThreads, 1) k_fp8_big(const __grid_constan
           const uint64_t adesc = sw128_desc(st), bdesc = sw128_desc(st + kFp8TileBytes);
           if (elected) {
 #pragma unroll
-            for (int kk = 0; kk < 4; ++kk) mma_f8(tmem + buf * 256, adesc + kk * 2, bdesc + kk * 2, idesc, kk > 0);
-            mma_commit(&d_full[buf]);
-            mma_commit(&empty[s]);
+            for (int kk = 0; kk < 4; ++kk) mma_f8_pair(tmem + buf * 256, adesc + kk * 2, bdesc + kk * 2, idesc, kk > 0);
+            mma_commit_pair(&d_full[buf]);
+            mma_commit_pair(&empty[s]);
           }
           if (++s == kBigStages) {
             s = 0;
@@ -780,13 +780,14 @@ __global__ void __launch_bounds__(kBigThreads, 1) k_fp8_big(const __grid_constan
           dph ^= buf == 0;
         }
       if (*abort_flag) {  // the MMAs in flight end before the tensor memory is freed
-        if (elected) mma_commit(drained);
+        if (elected) mma_commit_pair(drained);
         mbar_wait_bounded(drained, 0, p.err, AH_ETIMEOUT, kWaitLimit);
       }
     }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kBigRegsMany));
     const int q = warp & 3, h = (warp - 4) >> 2;  // TMEM lane quarter, column half
+    const uint32_t d_empty0 = mapa_shared(smem_u32(d_empty), 0);
     const uint32_t lane_addr = tmem + ((uint32_t)(q * 32) << 16) + h * 64;
     const bool vec = (reinterpret_cast<uintptr_t>(g.ascales) & 15) == 0 && g.lds % 4 == 0;
     const bool wvec = kb % 4 == 0;
@@ -795,7 +796,7 @@ __global__ void __launch_bounds__(kBigThreads, 1) k_fp8_big(const __grid_constan
     int buf = 0;
     uint32_t ph = 0;
     for (int tile = first; tile < tiles; tile += step) {
-      const int unit = tile / mt, m0 = tile % mt * kBigTokens + q * 32;
+      const int unit = tile / mt, m0 = tile % mt * kBigTokens + rank * 128 + q * 32;
       const int64_t tok = m0 + lane;
       const float* arow = g.ascales + (tok < g.m ? tok : 0) * g.lds;  // past m: stored nowhere
       const float* w0 = g.wscales + (int64_t)(unit * 2) * kb;
@@ -831,7 +832,7 @@ __global__ void __launch_bounds__(kBigThreads, 1) k_fp8_big(const __grid_constan
             } else {
               tc_fence_before();
               __syncwarp();
-              if (lane == 0) mbar_arrive(&d_empty[buf]);
+              if (lane == 0) mbar_arrive_cluster(d_empty0 + buf * 8);
             }
             const float f = c < 2 ? s0[i] : s1[i];
 #pragma unroll
@@ -932,9 +933,11 @@ __global__ void __launch_bounds__(kBigThreads, 1) k_fp8_big(const __grid_constan
 
   __syncwarp();
   __syncthreads();
+  cluster_arrive();
+  cluster_wait();
   if (warp == 1) {
     tc_fence_after();
-    tmem_dealloc(tmem, 512);
+    tmem_dealloc_pair(tmem, 512);
   }
 }
 
@@ -942,6 +945,9 @@ template <bool kGlu>
 int launch_big(BigArgs& p, cudaStream_t st) {
   const MatmulArgs& g = p.g;
   int rc = encode_rows(&p.tm_a, g.a, (uint64_t)g.cols, (uint64_t)g.m, (uint64_t)g.lda, 128);
+  if (rc != AH_OK) return rc;
+  rc = encode_2d(&p.tm_w, g.tiles, CU_TENSOR_MAP_DATA_TYPE_UINT8, 1, kFp8Group, (uint64_t)g.nt * g.kb * kFp8Group,
+                 kFp8Group, kFp8Group, CU_TENSOR_MAP_SWIZZLE_NONE);
   if (rc != AH_OK) return rc;
   const int elem = g.y_dtype == AH_DTYPE_F32 ? 4 : 2;
   p.y_map = !kGlu && !g.gate_up && aligned16(g.y) && g.ldy * elem % 16 == 0;
@@ -967,7 +973,7 @@ int launch_big(BigArgs& p, cudaStream_t st) {
   const int64_t tiles = (g.m + kBigTokens - 1) / kBigTokens * ((g.nt + 1) / 2);
   AH_REQUIRE(tiles < (1 << 30) && g.nt * g.kb < (1 << 24) && g.m <= 0x7FFFFF00,
              "fp8w_matmul: too many tiles for one launch");
-  return launch_pdl(k_fp8_big<kGlu>, dim3((unsigned)std::min<int64_t>(tiles, sm_count())), dim3(kBigThreads),
+  return launch_pdl(k_fp8_big<kGlu>, dim3((unsigned)(2 * std::min<int64_t>(tiles, sm_count() / 2))), dim3(kBigThreads),
                     Big::kDynamic, st, (const BigArgs)p);
 }
 
