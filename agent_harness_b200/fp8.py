@@ -14,7 +14,7 @@ import ctypes as C
 
 import torch
 
-from ._lib import AhError, call, lib
+from ._lib import AhError, call, check, lib
 
 GROUP = 128
 _DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 30}
@@ -25,19 +25,26 @@ def _refuse(message: str):
     raise AhError(-1, message)
 
 
-def _rows(t: torch.Tensor, what: str, like: torch.Tensor | None = None) -> int:
-    """The row stride of a CUDA matrix with unit-stride columns."""
-    if t.dim() != 2 or not t.is_cuda:
+# The checks below run on every call of a decode step, beside kernels of a few
+# microseconds: they read each tensor attribute once, and compare devices by index.
+
+def _rows(t: torch.Tensor, what: str, device: int | None = None) -> tuple[int, int, int]:
+    """(rows, columns, row stride) of a CUDA matrix with unit-stride columns."""
+    shape = t.shape
+    dev = t.get_device()
+    if len(shape) != 2 or dev < 0:
         _refuse(f"{what}: expected a CUDA matrix")
-    if like is not None and t.device != like.device:
+    if device is not None and dev != device:
         _refuse(f"{what}: on another device than the other tensors")
-    m, k = t.shape
-    if k > 1 and t.stride(1) != 1:
+    m, k = shape
+    ld, unit = t.stride()
+    if unit != 1 and k > 1:
         _refuse(f"{what}: expected unit-stride columns")
-    ld = t.stride(0) if m > 1 else max(k, t.stride(0))
     if ld < k:
-        _refuse(f"{what}: rows overlap")
-    return ld
+        if m > 1:
+            _refuse(f"{what}: rows overlap")
+        ld = k  # a single row's stride is free
+    return m, k, ld
 
 
 def _dtype(t: torch.Tensor, what: str) -> int:
@@ -47,17 +54,17 @@ def _dtype(t: torch.Tensor, what: str) -> int:
     return code
 
 
-def _quantised(q: torch.Tensor, scales: torch.Tensor, like: torch.Tensor | None = None) -> tuple[int, int]:
-    """Checks a (q, scales) pair; returns its row strides."""
-    ldq, lds = _rows(q, "q", like), _rows(scales, "scales", q)
-    if q.dtype != _E4M3 or scales.dtype != torch.float32:
+def _quantised(q: torch.Tensor, scales: torch.Tensor, device: int) -> tuple[int, int, int, int]:
+    """Checks a (q, scales) pair: (rows, columns, their row strides)."""
+    m, k, ldq = _rows(q, "q", device)
+    ms, ks, lds = _rows(scales, "scales", device)
+    if q.dtype is not _E4M3 or scales.dtype is not torch.float32:
         _refuse("expected q as float8_e4m3fn and scales as float32")
-    m, k = q.shape
-    if scales.shape[0] != m or scales.shape[1] != (k + GROUP - 1) // GROUP:
+    if ms != m or ks != (k + 127) // 128:
         _refuse("scales must be [rows, ceil(columns / 128)]")
-    if m <= 1:  # a single row's stride is free
+    if m <= 1:
         ldq = (ldq + 15) // 16 * 16
-    return ldq, lds
+    return m, k, ldq, lds
 
 
 def alloc(m: int, k: int, device="cuda") -> tuple[torch.Tensor, torch.Tensor]:
@@ -66,34 +73,45 @@ def alloc(m: int, k: int, device="cuda") -> tuple[torch.Tensor, torch.Tensor]:
     return q, torch.empty(m, (k + GROUP - 1) // GROUP, dtype=torch.float32, device=device)
 
 
-def _outputs(x: torch.Tensor, out, scales) -> tuple[torch.Tensor, torch.Tensor, int, int]:
-    m, k = x.shape
-    if (out is None) != (scales is None):
-        _refuse("give out and scales together")
+def _outputs(m: int, k: int, device: int, out, scales):
     if out is None:
-        out, scales = alloc(m, k, x.device)
-    elif out.shape != x.shape:
+        if scales is not None:
+            _refuse("give out and scales together")
+        out, scales = alloc(m, k, torch.device("cuda", device))
+        return out, scales, (k + 15) // 16 * 16, (k + 127) // 128
+    if scales is None:
+        _refuse("give out and scales together")
+    mo, ko, ldq, lds = _quantised(out, scales, device)
+    if mo != m or ko != k:
         _refuse("out must have the input's shape")
-    ldq, lds = _quantised(out, scales, x)
     return out, scales, ldq, lds
 
 
-def _run(device: torch.device, name: str, *args):
+_functions: dict = {}
+
+
+def _run(device: int, name: str, *args):
     """One library call on the device's current stream."""
-    if device.index == torch.cuda.current_device():
-        call(name, *args, torch.cuda.current_stream(device).cuda_stream)
+    fn = _functions.get(name)
+    if fn is None:
+        fn = _functions[name] = getattr(lib(), name)
+    stream = torch._C._cuda_getCurrentRawStream(device)
+    if torch._C._cuda_getDevice() == device:
+        rc = fn(*args, stream)
     else:
         with torch.cuda.device(device):
-            call(name, *args, torch.cuda.current_stream(device).cuda_stream)
+            rc = fn(*args, stream)
+    if rc:
+        check(rc)
 
 
 def quantize_fp8(x: torch.Tensor, out: torch.Tensor | None = None,
                  scales: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
     """x [m, k] f32 / f16 / bf16 -> (q, scales)."""
-    ldx, dt = _rows(x, "x"), _dtype(x, "x")
-    out, scales, ldq, lds = _outputs(x, out, scales)
-    m, k = x.shape
-    _run(x.device, "ah_fp8_quantize", x.data_ptr(), ldx, dt, m, k, out.data_ptr(), ldq, scales.data_ptr(), lds)
+    m, k, ldx = _rows(x, "x")
+    dt, dev = _dtype(x, "x"), x.get_device()
+    out, scales, ldq, lds = _outputs(m, k, dev, out, scales)
+    _run(dev, "ah_fp8_quantize", x.data_ptr(), ldx, dt, m, k, out.data_ptr(), ldq, scales.data_ptr(), lds)
     return out, scales
 
 
@@ -101,27 +119,29 @@ def swiglu_fp8(gate: torch.Tensor, up: torch.Tensor, out: torch.Tensor | None = 
                scales: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
     """silu(gate) * up (inference/ffn.rs:155-174), quantised: gate and up [m, k] of
     one type (halves of one matrix will do) -> (q, scales)."""
-    ldg, ldu, dt = _rows(gate, "gate"), _rows(up, "up", gate), _dtype(gate, "gate")
-    if up.shape != gate.shape or up.dtype != gate.dtype:
+    m, k, ldg = _rows(gate, "gate")
+    dt, dev = _dtype(gate, "gate"), gate.get_device()
+    mu, ku, ldu = _rows(up, "up", dev)
+    if mu != m or ku != k or up.dtype is not gate.dtype:
         _refuse("gate and up must have one shape and type")
-    out, scales, ldq, lds = _outputs(gate, out, scales)
-    m, k = gate.shape
-    _run(gate.device, "ah_fp8_swiglu", gate.data_ptr(), ldg, up.data_ptr(), ldu, dt, m, k, out.data_ptr(), ldq,
+    out, scales, ldq, lds = _outputs(m, k, dev, out, scales)
+    _run(dev, "ah_fp8_swiglu", gate.data_ptr(), ldg, up.data_ptr(), ldu, dt, m, k, out.data_ptr(), ldq,
          scales.data_ptr(), lds)
     return out, scales
 
 
 def _norm_args(x, norm_w, residual):
-    ldx, dt = _rows(x, "x"), _dtype(x, "x")
-    wdt = _dtype(norm_w, "norm_w")
-    if norm_w.shape != (x.shape[1],) or not norm_w.is_contiguous() or norm_w.device != x.device:
+    m, k, ldx = _rows(x, "x")
+    dt, dev, wdt = _dtype(x, "x"), x.get_device(), _dtype(norm_w, "norm_w")
+    if norm_w.shape != (k,) or not norm_w.is_contiguous() or norm_w.get_device() != dev:
         _refuse("norm_w must be one contiguous value per column, on x's device")
     rp, ldr = None, 0
     if residual is not None:
-        if residual.shape != x.shape or residual.dtype != x.dtype:
+        mr, kr, ldr = _rows(residual, "residual", dev)
+        if mr != m or kr != k or residual.dtype is not x.dtype:
             _refuse("residual must have x's shape and type")
-        rp, ldr = residual.data_ptr(), _rows(residual, "residual", x)
-    return ldx, dt, wdt, rp, ldr
+        rp = residual.data_ptr()
+    return m, k, dev, ldx, dt, wdt, rp, ldr
 
 
 def add_rms_norm_fp8(x: torch.Tensor, norm_w: torch.Tensor, residual: torch.Tensor | None = None, eps: float = 1e-5,
@@ -130,16 +150,15 @@ def add_rms_norm_fp8(x: torch.Tensor, norm_w: torch.Tensor, residual: torch.Tens
     """residual += x in place (no residual: x alone), then its RMS norm
     (inference/math.rs:53-63) times norm_w [k], quantised -> (q, scales).
     norm_w may be f16 (the decoder's storage), f32 or bf16."""
-    ldx, dt, wdt, rp, ldr = _norm_args(x, norm_w, residual)
-    out, scales, ldq, lds = _outputs(x, out, scales)
-    m, k = x.shape
-    _run(x.device, "ah_fp8_add_rms_norm", x.data_ptr(), ldx, rp, ldr, dt, norm_w.data_ptr(), wdt, eps, m, k,
+    m, k, dev, ldx, dt, wdt, rp, ldr = _norm_args(x, norm_w, residual)
+    out, scales, ldq, lds = _outputs(m, k, dev, out, scales)
+    _run(dev, "ah_fp8_add_rms_norm", x.data_ptr(), ldx, rp, ldr, dt, norm_w.data_ptr(), wdt, eps, m, k,
          out.data_ptr(), ldq, scales.data_ptr(), lds)
     return out, scales
 
 
 def _blocks_of(q: torch.Tensor, scales: torch.Tensor) -> tuple[int, int]:
-    ldq, lds = _rows(q, "q"), _rows(scales, "scales", q)
+    ldq, lds = _rows(q, "q")[2], _rows(scales, "scales", q.get_device())[2]
     if q.dtype != _E4M3 or scales.dtype != torch.float32:
         _refuse("expected q as float8_e4m3fn and scales as float32")
     if scales.shape != tuple((n + GROUP - 1) // GROUP for n in q.shape):
@@ -153,6 +172,7 @@ class Fp8Weight:
     def __init__(self, handle: C.c_void_p, rows: int, cols: int, device: torch.device):
         self._h = handle
         self.rows, self.cols, self.device = rows, cols, device
+        self._dev = device.index
 
     @classmethod
     def _make(cls, name: str, device: torch.device, rows: int, cols: int, *args, n: int | None = None) -> "Fp8Weight":
@@ -170,7 +190,7 @@ class Fp8Weight:
     @classmethod
     def from_float(cls, w: torch.Tensor) -> "Fp8Weight":
         """w [rows, cols] f32 / f16 / bf16, quantised on the device."""
-        ld, dt = _rows(w, "w"), _dtype(w, "w")
+        ld, dt = _rows(w, "w")[2], _dtype(w, "w")
         return cls._make("ah_fp8w_quantize", w.device, *w.shape, w.data_ptr(), ld, dt)
 
     @property
@@ -184,17 +204,16 @@ class Fp8Weight:
     def matmul(self, q: torch.Tensor, scales: torch.Tensor, out: torch.Tensor | None = None,
                dtype: torch.dtype = torch.float32) -> torch.Tensor:
         """y = dequant(q, scales) @ W^T, [m, rows] in out's type (or dtype), sums in f32."""
-        ldq, lds = _quantised(q, scales)
-        if q.shape[1] != self.cols or q.device != self.device:
-            _refuse(f"q must be [m, {self.cols}] on {self.device}")
-        m = q.shape[0]
+        m, k, ldq, lds = _quantised(q, scales, self._dev)
+        if k != self.cols:
+            _refuse(f"q must be [m, {self.cols}]")
         if out is None:
-            out = torch.empty(m, self.rows, dtype=dtype, device=q.device)
-        elif out.shape != (m, self.rows):
+            out = torch.empty(m, self.rows, dtype=dtype, device=self.device)
+        my, ny, ldy = _rows(out, "out", self._dev)
+        if my != m or ny != self.rows:
             _refuse(f"out must be [{m}, {self.rows}]")
-        ldy, dt = _rows(out, "out", q), _dtype(out, "out")
-        _run(self.device, "ah_fp8w_matmul", self._h, q.data_ptr(), ldq, scales.data_ptr(), lds, m, out.data_ptr(), ldy,
-             dt)
+        _run(self._dev, "ah_fp8w_matmul", self._h, q.data_ptr(), ldq, scales.data_ptr(), lds, m, out.data_ptr(), ldy,
+             _dtype(out, "out"))
         return out
 
     def close(self):
@@ -217,6 +236,8 @@ class Fp8SwigluBlock:
     def __init__(self, gate_up: Fp8Weight, down: Fp8Weight):
         self.gate_up, self.down = gate_up, down
         self.n_embd, self.n_ff, self.device = down.rows, down.cols, down.device
+        self._dev = down.device.index
+        self._bytes = (-1, 0)  # rows and workspace bytes of the last call
 
     @staticmethod
     def _check(gate, up, down):
@@ -240,7 +261,7 @@ class Fp8SwigluBlock:
     def from_float(cls, gate: torch.Tensor, up: torch.Tensor, down: torch.Tensor) -> "Fp8SwigluBlock":
         """The same from f32 / f16 / bf16 matrices, quantised on the device."""
         cls._check(gate, up, down)
-        ldg, ldu, dt = _rows(gate, "gate"), _rows(up, "up"), _dtype(gate, "gate")
+        ldg, ldu, dt = _rows(gate, "gate")[2], _rows(up, "up")[2], _dtype(gate, "gate")
         n_ff, n_embd = gate.shape
         dn = Fp8Weight.from_float(down)
         gate_up = Fp8Weight._make("ah_fp8w_quantize_gate_up", gate.device, 2 * n_ff, n_embd, gate.data_ptr(), ldg,
@@ -257,18 +278,21 @@ class Fp8SwigluBlock:
         """x [m, n_embd] -> the block's output [m, n_embd] in x's type (or out's);
         residual += x in place.  The caller, or the next norm, adds the output to
         the residual."""
-        ldx, dt, wdt, rp, ldr = _norm_args(x, norm_w, residual)
-        if x.shape[1] != self.n_embd or x.device != self.device:
+        m, k, dev, ldx, dt, wdt, rp, ldr = _norm_args(x, norm_w, residual)
+        if k != self.n_embd or dev != self._dev:
             _refuse(f"x must be [m, {self.n_embd}] on {self.device}")
         if out is None:
-            out = torch.empty(x.shape, dtype=x.dtype, device=x.device)
-        elif out.shape != x.shape:
+            out = torch.empty(m, k, dtype=x.dtype, device=self.device)
+        my, ny, ldy = _rows(out, "out", dev)
+        if my != m or ny != k:
             _refuse("out must have x's shape")
-        ldy, odt = _rows(out, "out", x), _dtype(out, "out")
-        m = x.shape[0]
-        ws = torch.empty(self.workspace_bytes(m), dtype=torch.uint8, device=x.device)
-        _run(self.device, "ah_fp8_ffn", self.gate_up.handle, self.down.handle, x.data_ptr(), ldx, rp, ldr, dt,
-             norm_w.data_ptr(), wdt, eps, m, out.data_ptr(), ldy, odt, ws.data_ptr(), ws.numel())
+        rows, nbytes = self._bytes
+        if rows != m:
+            nbytes = self.workspace_bytes(m)
+            self._bytes = (m, nbytes)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=self.device)
+        _run(dev, "ah_fp8_ffn", self.gate_up.handle, self.down.handle, x.data_ptr(), ldx, rp, ldr, dt,
+             norm_w.data_ptr(), wdt, eps, m, out.data_ptr(), ldy, _dtype(out, "out"), ws.data_ptr(), nbytes)
         return out
 
     def close(self):
