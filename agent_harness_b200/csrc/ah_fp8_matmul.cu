@@ -116,7 +116,7 @@ __global__ void __launch_bounds__(256) k_fp8w_quantize(const BuildArgs g) {
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < 8; ++i) a = max(a, red[i]);
-    const float gm = __uint_as_float(a), inv = __fdiv_rn(kFp8Max, gm);
+    const float gm = __uint_as_float(a), inv = fp8_inverse(gm);
     uint8_t* dst = g.tiles + fp8_image(g.gate_up, g.kb, t, b) * kFp8TileBytes;
 #pragma unroll
     for (int i = 0; i < 4; ++i) {
@@ -513,13 +513,10 @@ __global__ void __launch_bounds__(kSmallThreads, 2) k_fp8_small(const __grid_con
           up[0] += __uint_as_float(b.x); up[1] += __uint_as_float(b.y);
           up[2] += __uint_as_float(b.z); up[3] += __uint_as_float(b.w);
         }
-        uint32_t mx = __float_as_uint(kFp8Tiny);
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-          gt[i] = r + i < n_ff ? fp8_silu_mul(gt[i], up[i]) : 0.0f;
-          mx = max(mx, __float_as_uint(gt[i]) & 0x7FFFFFFFu);
-        }
-        const float gm = __uint_as_float(__reduce_max_sync(0xFFFFFFFFu, mx)), inv = __fdiv_rn(kFp8Max, gm);
+        for (int i = 0; i < 4; ++i) gt[i] = r + i < n_ff ? fp8_silu_mul(gt[i], up[i]) : 0.0f;
+        const float fm = max_abs3(max_abs3(kFp8Tiny, gt[0], gt[1]), gt[2], gt[3]);
+        const float gm = __uint_as_float(__reduce_max_sync(0xFFFFFFFFu, __float_as_uint(fm))), inv = fp8_inverse(gm);
         const uint32_t w = cvt_e4m3x4(gt[0] * inv, gt[1] * inv, gt[2] * inv, gt[3] * inv);
         uint8_t* qrow = p.act_q + (m0 + c) * p.ld_act + r;  // ld_act is a multiple of 16
         if (r + 4 <= n_ff) *reinterpret_cast<uint32_t*>(qrow) = w;
@@ -660,10 +657,6 @@ __device__ __forceinline__ void load_scales4(const float* row, int b, int kb, bo
     for (int i = 0; i < 4; ++i) v[i] = b + i < kb ? row[b + i] : 0.0f;
   }
 }
-
-// silu(g) * u with the fast exponential and division: the product is rounded to
-// 4 significant bits next, a relative error of about 2^-20 moves one in 10^5.
-__device__ __forceinline__ float fp8_silu_mul_fast(float g, float u) { return __fdividef(g, 1.0f + __expf(-g)) * u; }
 
 template <typename T>
 __device__ __forceinline__ uint32_t pack2(float a, float b);
@@ -848,19 +841,21 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kBigThreads, 1) k_fp
       const bool ok = !__any_sync(0xFFFFFFFFu, *abort_flag);  // after a give-up nothing is stored
       if constexpr (kGlu) {
         const int64_t n_ff = g.rows / 2, c0 = (int64_t)unit * kFp8Group + h * 64;
-        uint32_t mx = __float_as_uint(kFp8Tiny);
+        float fm = kFp8Tiny;
 #pragma unroll
-        for (int j = 0; j < 64; ++j) {
+        for (int j = 0; j < 64; j += 2) {
           // rows past n_ff are zero in the images: their products are zero
-          acc[0][j] = fp8_silu_mul_fast(acc[0][j], acc[1][j]);
-          mx = max(mx, __float_as_uint(acc[0][j]) & 0x7FFFFFFFu);
+          acc[0][j] = fp8_silu_mul(acc[0][j], acc[1][j]);
+          acc[0][j + 1] = fp8_silu_mul(acc[0][j + 1], acc[1][j + 1]);
+          fm = max_abs3(fm, acc[0][j], acc[0][j + 1]);
         }
+        uint32_t mx = __float_as_uint(fm);  // a NaN's bits are above every number's
         uint32_t* maxima = reinterpret_cast<uint32_t*>(smem + Big::kMax);
         maxima[h * 128 + q * 32 + lane] = mx;
         asm volatile("bar.sync 1, 256;" ::: "memory");
         mx = max(mx, maxima[(h ^ 1) * 128 + q * 32 + lane]);
         asm volatile("bar.sync 1, 256;" ::: "memory");  // read before the next tile writes
-        const float gm = __uint_as_float(mx), inv = __fdiv_rn(kFp8Max, gm);
+        const float gm = __uint_as_float(mx), inv = fp8_inverse(gm);
         if (ok && tok < g.m) {
           uint8_t* qrow = p.act_q + tok * p.ld_act + c0;  // 16-byte aligned: ld_act is a multiple of 16
 #pragma unroll

@@ -12,8 +12,10 @@
 // its data, without waiting for the row's sum.  All arithmetic is f32; each z
 // is rounded once, to e4m3.
 //
-// A group's maximum is taken on the bits of |z|, where a NaN is above every
-// number: a group with a NaN or an infinity comes out as NaN.
+// A group's maximum keeps a NaN, and an infinite one has a NaN inverse: a group
+// with a NaN or an infinity comes out as NaN.
+#include <algorithm>
+
 #include "ah_common.cuh"
 #include "ah_fp8.cuh"
 #include "ah_sm100.cuh"
@@ -42,56 +44,54 @@ __device__ __forceinline__ __half from_f32<__half>(float v) { return __float2hal
 template <>
 __device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
 
-// Columns [c, c + kV) of a row of k columns (zero past it).  `vec`: row + c is
-// 16-byte aligned and the piece lies inside the row.
-template <typename T>
-__device__ __forceinline__ void load_piece(const T* row, int64_t c, int64_t k, bool vec, float (&v)[Vec<T>::kV]) {
-  if (vec) {
-    const uint4 p = *reinterpret_cast<const uint4*>(row + c);
-    const T* e = reinterpret_cast<const T*>(&p);
-#pragma unroll
-    for (int i = 0; i < Vec<T>::kV; ++i) v[i] = to_f32(e[i]);
-  } else {
-#pragma unroll
-    for (int i = 0; i < Vec<T>::kV; ++i) v[i] = c + i < k ? to_f32(row[c + i]) : 0.0f;
+// Columns [c, c + kV) of a row of k columns as its 16 bytes (zero past the row).
+// kVec: rows start at multiples of 16 bytes and k is a multiple of kV.
+template <bool kVec, typename T>
+__device__ __forceinline__ uint4 load_piece(const T* row, int c, int k) {
+  uint4 p = make_uint4(0, 0, 0, 0);
+  if constexpr (kVec) {
+    if (c < k) p = *reinterpret_cast<const uint4*>(row + c);
+    return p;
   }
+  T* e = reinterpret_cast<T*>(&p);
+#pragma unroll
+  for (int i = 0; i < Vec<T>::kV; ++i)
+    if (c + i < k) e[i] = row[c + i];
+  return p;
 }
 
 template <typename T>
-__device__ __forceinline__ void store_piece(T* row, int64_t c, int64_t k, bool vec, const float (&v)[Vec<T>::kV]) {
-  if (vec) {
-    uint4 p;
-    T* e = reinterpret_cast<T*>(&p);
+__device__ __forceinline__ void unpack(const uint4& p, float (&v)[Vec<T>::kV]) {
+  const T* e = reinterpret_cast<const T*>(&p);
 #pragma unroll
-    for (int i = 0; i < Vec<T>::kV; ++i) e[i] = from_f32<T>(v[i]);
-    *reinterpret_cast<uint4*>(row + c) = p;
-  } else {
-#pragma unroll
-    for (int i = 0; i < Vec<T>::kV; ++i)
-      if (c + i < k) row[c + i] = from_f32<T>(v[i]);
-  }
+  for (int i = 0; i < Vec<T>::kV; ++i) v[i] = to_f32(e[i]);
 }
 
 // The group maximum of |z| (at least 2^-100) over the group's lanes.
 template <typename T>
 __device__ __forceinline__ float group_max(const float (&z)[Vec<T>::kV]) {
-  uint32_t a = __float_as_uint(kFp8Tiny);
+  float f = kFp8Tiny;
 #pragma unroll
-  for (int i = 0; i < Vec<T>::kV; ++i) a = max(a, __float_as_uint(z[i]) & 0x7FFFFFFFu);
+  for (int i = 0; i < Vec<T>::kV; i += 2) f = max_abs3(f, z[i], z[i + 1]);
+  uint32_t a = __float_as_uint(f);  // a NaN's bits are above every number's
+  if constexpr (Vec<T>::kLanes == 32) {
+    a = __reduce_max_sync(0xFFFFFFFFu, a);
+  } else {
 #pragma unroll
-  for (int o = Vec<T>::kLanes / 2; o; o >>= 1) a = max(a, __shfl_xor_sync(0xFFFFFFFFu, a, o));
+    for (int o = Vec<T>::kLanes / 2; o; o >>= 1) a = max(a, __shfl_xor_sync(0xFFFFFFFFu, a, o));
+  }
   return __uint_as_float(a);
 }
 
 // q bytes of columns [c, c + kV): one 4- or 8-byte store (ldq and q are
 // multiples of 16 bytes), bytes at the end of a ragged row.
-template <int kV>
-__device__ __forceinline__ void store_q(uint8_t* qrow, int64_t c, int64_t k, const float (&z)[kV], float inv) {
+template <bool kVec, int kV>
+__device__ __forceinline__ void store_q(uint8_t* qrow, int c, int k, const float (&z)[kV], float inv) {
   uint32_t w[kV / 4];
 #pragma unroll
   for (int i = 0; i < kV / 4; ++i)
     w[i] = cvt_e4m3x4(z[4 * i] * inv, z[4 * i + 1] * inv, z[4 * i + 2] * inv, z[4 * i + 3] * inv);
-  if (c + kV <= k) {
+  if (kVec || c + kV <= k) {
     if constexpr (kV == 4)
       *reinterpret_cast<uint32_t*>(qrow + c) = w[0];
     else
@@ -107,35 +107,50 @@ struct RowArgs {
   const void* a;  // x, or gate
   const void* b;  // up
   int64_t lda, ldb;
-  int64_t m, k;
+  int64_t m;
+  int k;
   uint8_t* q;
   int64_t ldq;
   float* scales;
   int64_t lds;
-  bool vec;  // a and b rows start at multiples of 16 bytes
 };
 
 constexpr int kRowThreads = 256;
 
-// One CTA per row and 256 * kV columns.
-template <int kMode, typename T>
+// One CTA per row and 256 * kN * kV columns: a thread requests its kN pieces of
+// every input before it uses the first.
+template <int kMode, typename T, bool kVec, int kN>
 __global__ void __launch_bounds__(kRowThreads) k_fp8_rows(const RowArgs g) {
   constexpr int kV = Vec<T>::kV;
-  const int64_t c = ((int64_t)blockIdx.x * kRowThreads + threadIdx.x) * kV;
+  pdl_launch_dependents();
+  pdl_wait();
+  const int c0 = (int)(blockIdx.x * kN * kRowThreads + threadIdx.x) * kV;
   for (int64_t row = blockIdx.y; row < g.m; row += gridDim.y) {
-    const bool vec = g.vec && c + kV <= g.k;
-    float z[kV];
-    load_piece(static_cast<const T*>(g.a) + row * g.lda, c, g.k, vec, z);
-    if (kMode == kRowSwiglu) {
-      float u[kV];
-      load_piece(static_cast<const T*>(g.b) + row * g.ldb, c, g.k, vec, u);
+    const T* arow = static_cast<const T*>(g.a) + row * g.lda;
+    const T* brow = static_cast<const T*>(g.b) + row * g.ldb;
+    uint4 pa[kN], pb[kMode == kRowSwiglu ? kN : 1];
 #pragma unroll
-      for (int i = 0; i < kV; ++i) z[i] = fp8_silu_mul(z[i], u[i]);
+    for (int i = 0; i < kN; ++i) {
+      const int c = c0 + i * kRowThreads * kV;
+      pa[i] = load_piece<kVec>(arow, c, g.k);
+      if constexpr (kMode == kRowSwiglu) pb[i] = load_piece<kVec>(brow, c, g.k);
     }
-    const float gm = group_max<T>(z);
-    if (c < g.k) {
-      store_q<kV>(g.q + row * g.ldq, c, g.k, z, __fdiv_rn(kFp8Max, gm));
-      if (c % kFp8Group == 0) g.scales[row * g.lds + c / kFp8Group] = gm * (1.0f / kFp8Max);
+#pragma unroll
+    for (int i = 0; i < kN; ++i) {
+      const int c = c0 + i * kRowThreads * kV;
+      float z[kV];
+      unpack<T>(pa[i], z);
+      if constexpr (kMode == kRowSwiglu) {
+        float u[kV];
+        unpack<T>(pb[i], u);
+#pragma unroll
+        for (int j = 0; j < kV; ++j) z[j] = fp8_silu_mul(z[j], u[j]);
+      }
+      const float gm = group_max<T>(z);
+      if (c < g.k) {
+        store_q<kVec>(g.q + row * g.ldq, c, g.k, z, fp8_inverse(gm));
+        if (c % kFp8Group == 0) g.scales[row * g.lds + c / kFp8Group] = gm * (1.0f / kFp8Max);
+      }
     }
   }
 }
@@ -145,71 +160,152 @@ struct NormArgs {
   void* residual;
   const void* w;
   int64_t ldx, ldr;
-  int64_t m, k;
+  int64_t m;
+  int k;
   uint8_t* q;
   int64_t ldq;
   float* scales;
   int64_t lds;
   uint32_t w_dtype;
   float eps;
-  bool vec;  // x, residual and w rows start at multiples of 16 bytes
 };
 
-__device__ __forceinline__ float norm_weight(const void* w, uint32_t dtype, int64_t c) {
-  if (dtype == AH_DTYPE_F32) return static_cast<const float*>(w)[c];
-  const unsigned short b = static_cast<const unsigned short*>(w)[c];
-  return dtype == AH_DTYPE_F16 ? __half2float(__ushort_as_half(b)) : __uint_as_float((uint32_t)b << 16);
-}
-
-// One CTA per row.
-template <typename T>
-__global__ void __launch_bounds__(kRowThreads) k_fp8_norm(const NormArgs g) {
-  constexpr int kV = Vec<T>::kV;
-  __shared__ float red[kRowThreads / 32];
-  const int64_t row = blockIdx.x;
-  float* scales = g.scales + row * g.lds;
-  float ss = 0.0f;
-  const int64_t sweep = (int64_t)kRowThreads * kV;
-  for (int64_t c0 = 0; c0 < g.k; c0 += sweep) {
-    const int64_t c = c0 + (int64_t)threadIdx.x * kV;
-    const bool vec = g.vec && c + kV <= g.k;
-    float h[kV];
-    load_piece(static_cast<const T*>(g.x) + row * g.ldx, c, g.k, vec, h);
-    if (g.residual) {
-      T* rrow = static_cast<T*>(g.residual) + row * g.ldr;
-      float r[kV];
-      load_piece<T>(rrow, c, g.k, vec, r);
+// Norm weights of columns [c, c + kV) (kVec: w is 16-byte aligned too).
+template <bool kVec, int kV>
+__device__ __forceinline__ void norm_weights(const NormArgs& g, int c, float (&w)[kV]) {
+  if constexpr (kVec) {
+    if (c >= g.k) {
 #pragma unroll
-      for (int i = 0; i < kV; ++i) h[i] = to_f32(from_f32<T>(h[i] + r[i]));
-      store_piece(rrow, c, g.k, vec, h);
+      for (int i = 0; i < kV; ++i) w[i] = 0.0f;
+      return;
     }
+    if (g.w_dtype == AH_DTYPE_F32) {
+#pragma unroll
+      for (int i = 0; i < kV; i += 4) {
+        const float4 f = *reinterpret_cast<const float4*>(static_cast<const float*>(g.w) + c + i);
+        w[i] = f.x; w[i + 1] = f.y; w[i + 2] = f.z; w[i + 3] = f.w;
+      }
+    } else {
+      uint32_t b[kV / 2];
+      const unsigned short* p = static_cast<const unsigned short*>(g.w) + c;
+      if constexpr (kV == 4) {
+        const uint2 v = *reinterpret_cast<const uint2*>(p);
+        b[0] = v.x; b[1] = v.y;
+      } else {
+        const uint4 v = *reinterpret_cast<const uint4*>(p);
+        b[0] = v.x; b[1] = v.y; b[2] = v.z; b[3] = v.w;
+      }
+#pragma unroll
+      for (int i = 0; i < kV / 2; ++i) {
+        const float2 f = g.w_dtype == AH_DTYPE_F16
+                             ? __half22float2(*reinterpret_cast<const __half2*>(&b[i]))
+                             : make_float2(__uint_as_float(b[i] << 16), __uint_as_float(b[i] & 0xFFFF0000u));
+        w[2 * i] = f.x;
+        w[2 * i + 1] = f.y;
+      }
+    }
+  } else {
 #pragma unroll
     for (int i = 0; i < kV; ++i) {
-      ss = fmaf(h[i], h[i], ss);
-      h[i] *= c + i < g.k ? norm_weight(g.w, g.w_dtype, c + i) : 0.0f;
+      if (c + i >= g.k) {
+        w[i] = 0.0f;
+      } else if (g.w_dtype == AH_DTYPE_F32) {
+        w[i] = static_cast<const float*>(g.w)[c + i];
+      } else {
+        const unsigned short b = static_cast<const unsigned short*>(g.w)[c + i];
+        w[i] = g.w_dtype == AH_DTYPE_F16 ? __half2float(__ushort_as_half(b)) : __uint_as_float((uint32_t)b << 16);
+      }
     }
-    const float gm = group_max<T>(h);
-    if (c < g.k) {
-      store_q<kV>(g.q + row * g.ldq, c, g.k, h, __fdiv_rn(kFp8Max, gm));
-      if (c % kFp8Group == 0) scales[c / kFp8Group] = gm * (1.0f / kFp8Max);  // times r below
+  }
+}
+
+// One row per threadIdx.y: blockDim.x threads take kN pieces each per sweep (one
+// sweep for most widths).  Several rows share a CTA only where a warp takes a row.
+template <typename T, bool kVec, int kN>
+__global__ void __launch_bounds__(kN == 1 ? 1024 : 512, kN == 1 ? 1 : 2) k_fp8_norm(const NormArgs g) {
+  constexpr int kV = Vec<T>::kV;
+  __shared__ float red[32];
+  pdl_launch_dependents();
+  pdl_wait();
+  const int64_t row = (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
+  if (row >= g.m) return;  // a whole warp: CTAs of one row have no such row
+  const T* xrow = static_cast<const T*>(g.x) + row * g.ldx;
+  T* rrow = g.residual ? static_cast<T*>(g.residual) + row * g.ldr : nullptr;
+  float* scales = g.scales + row * g.lds;
+  const int sweep = (int)blockDim.x * kN * kV;
+  float ss = 0.0f, gm[kN];
+  for (int s = 0; s < g.k; s += sweep) {
+    uint4 px[kN], pr[kN];
+#pragma unroll
+    for (int i = 0; i < kN; ++i) {
+      const int c = s + (int)(i * blockDim.x + threadIdx.x) * kV;
+      px[i] = load_piece<kVec>(xrow, c, g.k);
+      if (rrow) pr[i] = load_piece<kVec, T>(rrow, c, g.k);
+    }
+#pragma unroll
+    for (int i = 0; i < kN; ++i) {
+      const int c = s + (int)(i * blockDim.x + threadIdx.x) * kV;
+      float h[kV], w[kV];
+      unpack<T>(px[i], h);
+      if (rrow) {
+        float r[kV];
+        unpack<T>(pr[i], r);
+        uint4 p;
+        T* e = reinterpret_cast<T*>(&p);
+#pragma unroll
+        for (int j = 0; j < kV; ++j) {
+          e[j] = from_f32<T>(h[j] + r[j]);
+          h[j] = to_f32(e[j]);
+        }
+        if constexpr (kVec) {
+          if (c < g.k) *reinterpret_cast<uint4*>(rrow + c) = p;
+        } else {
+#pragma unroll
+          for (int j = 0; j < kV; ++j)
+            if (c + j < g.k) rrow[c + j] = e[j];
+        }
+      }
+      norm_weights<kVec>(g, c, w);
+#pragma unroll
+      for (int j = 0; j < kV; ++j) {
+        ss = fmaf(h[j], h[j], ss);
+        h[j] *= w[j];
+      }
+      gm[i] = group_max<T>(h);
+      if (c < g.k) {
+        store_q<kVec>(g.q + row * g.ldq, c, g.k, h, fp8_inverse(gm[i]));
+        // more than one sweep: the maximum waits for r in the scales themselves
+        if (sweep < g.k && c % kFp8Group == 0) scales[c / kFp8Group] = gm[i];
+      }
     }
   }
 #pragma unroll
   for (int o = 16; o; o >>= 1) ss += __shfl_xor_sync(0xFFFFFFFFu, ss, o);
-  if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = ss;
-  __syncthreads();
-  ss = red[0];
+  if (blockDim.x > 32) {
+    if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = ss;
+    __syncthreads();
+    // every warp adds the partial sums in the same order
+    ss = threadIdx.x % 32 < blockDim.x / 32 ? red[threadIdx.x & 31] : 0.0f;
 #pragma unroll
-  for (int i = 1; i < kRowThreads / 32; ++i) ss += red[i];
-  const float r = __fdiv_rn(1.0f, sqrtf(__fdiv_rn(ss, (float)g.k) + g.eps));
-  for (int64_t c = (int64_t)threadIdx.x * kV; c < g.k; c += sweep)
-    if (c % kFp8Group == 0) scales[c / kFp8Group] *= r;  // this thread's own store
+    for (int o = 16; o; o >>= 1) ss += __shfl_xor_sync(0xFFFFFFFFu, ss, o);
+  }
+  const float r = __fdiv_rn(1.0f, sqrtf(__fdiv_rn(ss, (float)g.k) + g.eps)) * (1.0f / kFp8Max);
+  if (sweep >= g.k) {
+#pragma unroll
+    for (int i = 0; i < kN; ++i) {
+      const int c = (int)(i * blockDim.x + threadIdx.x) * kV;
+      if (c < g.k && c % kFp8Group == 0) scales[c / kFp8Group] = gm[i] * r;
+    }
+  } else {
+    for (int c = (int)threadIdx.x * kV; c < g.k; c += (int)blockDim.x * kV)
+      if (c % kFp8Group == 0) scales[c / kFp8Group] *= r;  // this thread's own store
+  }
 }
 
 int check_rows(const char* who, int64_t m, int64_t k, const void* q, int64_t ldq, const void* scales, int64_t lds,
                uint32_t dtype) {
   AH_REQUIRE(m >= 0 && k >= 1, "%s: needs m >= 0 rows of k >= 1 columns", who);
-  AH_REQUIRE(m <= 0x7FFFFFFF && k <= 0x7FFFFFFF, "%s: m and k must be below 2^31", who);
+  AH_REQUIRE(m <= 0x7FFFFFFF && k < (1 << 30), "%s: m must be below 2^31 and k below 2^30", who);
   AH_REQUIRE(dtype == AH_DTYPE_F32 || dtype == AH_DTYPE_F16 || dtype == AH_DTYPE_BF16,
              "%s: dtype %u is not f32, f16 or bf16", who, dtype);
   AH_REQUIRE(m == 0 || (q && scales), "%s: null pointer", who);
@@ -224,26 +320,36 @@ bool vec_rows(const void* p, int64_t ld, uint32_t dtype) {
 }
 
 template <int kMode, typename T>
-int launch_rows(const RowArgs& g, cudaStream_t st) {
-  const int64_t cols = (int64_t)kRowThreads * Vec<T>::kV;
-  const dim3 grid((unsigned)((g.k + cols - 1) / cols), (unsigned)(g.m < 65535 ? g.m : 65535));
-  k_fp8_rows<kMode, T><<<grid, kRowThreads, 0, st>>>(g);
-  AH_LAUNCH_CHECK();
-  return AH_OK;
+int launch_rows(const RowArgs& g, bool vec, cudaStream_t st) {
+  // two pieces per thread once that still leaves every SM four CTAs
+  const int64_t pieces = (g.k + Vec<T>::kV - 1) / Vec<T>::kV;
+  vec = vec && g.k % Vec<T>::kV == 0;
+  const bool many = vec && g.m * ((pieces + 2 * kRowThreads - 1) / (2 * kRowThreads)) >= 4 * (int64_t)sm_count();
+  const int64_t cols = (int64_t)kRowThreads * (many ? 2 : 1);
+  const dim3 grid((unsigned)((pieces + cols - 1) / cols), (unsigned)(g.m < 65535 ? g.m : 65535));
+  return launch_pdl(many ? k_fp8_rows<kMode, T, true, 2> : vec ? k_fp8_rows<kMode, T, true, 1> : k_fp8_rows<kMode, T, false, 1>,
+                    grid, dim3(kRowThreads), 0, st, g);
 }
 
 template <int kMode>
-int dispatch_rows(const RowArgs& g, uint32_t dtype, cudaStream_t st) {
-  if (dtype == AH_DTYPE_F32) return launch_rows<kMode, float>(g, st);
-  if (dtype == AH_DTYPE_F16) return launch_rows<kMode, __half>(g, st);
-  return launch_rows<kMode, __nv_bfloat16>(g, st);
+int dispatch_rows(const RowArgs& g, uint32_t dtype, bool vec, cudaStream_t st) {
+  if (dtype == AH_DTYPE_F32) return launch_rows<kMode, float>(g, vec, st);
+  if (dtype == AH_DTYPE_F16) return launch_rows<kMode, __half>(g, vec, st);
+  return launch_rows<kMode, __nv_bfloat16>(g, vec, st);
 }
 
 template <typename T>
-int launch_norm(const NormArgs& g, cudaStream_t st) {
-  k_fp8_norm<T><<<(unsigned)g.m, kRowThreads, 0, st>>>(g);
-  AH_LAUNCH_CHECK();
-  return AH_OK;
+int launch_norm(const NormArgs& g, bool vec, cudaStream_t st) {
+  // Few rows: one piece per thread, up to 1024 threads, for the latency of one
+  // round of loads.  Many rows: four pieces per thread (a warp per row where that
+  // covers it), for few threads per row and many rows in flight.
+  const int64_t pieces = (g.k + Vec<T>::kV - 1) / Vec<T>::kV;
+  vec = vec && g.k % Vec<T>::kV == 0;
+  const int n = g.m > 2 * (int64_t)sm_count() && vec ? 4 : 1;
+  const unsigned tx = (unsigned)std::min<int64_t>(n == 1 ? 1024 : 512, ((pieces + n - 1) / n + 31) / 32 * 32);
+  const unsigned ty = tx == 32 ? 8 : 1;
+  return launch_pdl(n == 4 ? k_fp8_norm<T, true, 4> : vec ? k_fp8_norm<T, true, 1> : k_fp8_norm<T, false, 1>,
+                    dim3((unsigned)((g.m + ty - 1) / ty)), dim3(tx, ty), 0, st, g);
 }
 
 }  // namespace
@@ -258,8 +364,8 @@ int ah_fp8_quantize(const void* x, int64_t ldx, uint32_t dtype, int64_t m, int64
   const int rc = check_rows("fp8_quantize", m, k, q, ldq, scales, lds, dtype);
   if (rc != AH_OK || m == 0) return rc;
   AH_REQUIRE(x && ldx >= k, "fp8_quantize: null x or ldx below k");
-  RowArgs g{x, nullptr, ldx, 0, m, k, q, ldq, scales, lds, vec_rows(x, ldx, dtype)};
-  return dispatch_rows<kRowQuantize>(g, dtype, as_stream(stream));
+  const RowArgs g{x, nullptr, ldx, 0, m, (int)k, q, ldq, scales, lds};
+  return dispatch_rows<kRowQuantize>(g, dtype, vec_rows(x, ldx, dtype), as_stream(stream));
 }
 
 int ah_fp8_swiglu(const void* gate, int64_t ld_gate, const void* up, int64_t ld_up, uint32_t dtype, int64_t m,
@@ -267,9 +373,9 @@ int ah_fp8_swiglu(const void* gate, int64_t ld_gate, const void* up, int64_t ld_
   const int rc = check_rows("fp8_swiglu", m, k, q, ldq, scales, lds, dtype);
   if (rc != AH_OK || m == 0) return rc;
   AH_REQUIRE(gate && up && ld_gate >= k && ld_up >= k, "fp8_swiglu: null input or a row stride below k");
-  RowArgs g{gate, up, ld_gate, ld_up, m, k, q, ldq, scales, lds,
-            vec_rows(gate, ld_gate, dtype) && vec_rows(up, ld_up, dtype)};
-  return dispatch_rows<kRowSwiglu>(g, dtype, as_stream(stream));
+  const RowArgs g{gate, up, ld_gate, ld_up, m, (int)k, q, ldq, scales, lds};
+  return dispatch_rows<kRowSwiglu>(g, dtype, vec_rows(gate, ld_gate, dtype) && vec_rows(up, ld_up, dtype),
+                                   as_stream(stream));
 }
 
 int ah_fp8_add_rms_norm(const void* x, int64_t ldx, void* residual, int64_t ldr, uint32_t dtype, const void* norm_w,
@@ -282,11 +388,11 @@ int ah_fp8_add_rms_norm(const void* x, int64_t ldx, void* residual, int64_t ldr,
   AH_REQUIRE(norm_dtype == AH_DTYPE_F32 || norm_dtype == AH_DTYPE_F16 || norm_dtype == AH_DTYPE_BF16,
              "fp8_add_rms_norm: norm weight dtype %u is not f32, f16 or bf16", norm_dtype);
   AH_REQUIRE(eps >= 0.0f, "fp8_add_rms_norm: eps must be >= 0");
-  NormArgs g{x, residual, norm_w, ldx, ldr, m, k, q, ldq, scales, lds, norm_dtype, eps,
-             vec_rows(x, ldx, dtype) && (!residual || vec_rows(residual, ldr, dtype))};
-  if (dtype == AH_DTYPE_F32) return launch_norm<float>(g, as_stream(stream));
-  if (dtype == AH_DTYPE_F16) return launch_norm<__half>(g, as_stream(stream));
-  return launch_norm<__nv_bfloat16>(g, as_stream(stream));
+  const NormArgs g{x, residual, norm_w, ldx, ldr, m, (int)k, q, ldq, scales, lds, norm_dtype, eps};
+  const bool vec = vec_rows(x, ldx, dtype) && (!residual || vec_rows(residual, ldr, dtype)) && aligned16(norm_w);
+  if (dtype == AH_DTYPE_F32) return launch_norm<float>(g, vec, as_stream(stream));
+  if (dtype == AH_DTYPE_F16) return launch_norm<__half>(g, vec, as_stream(stream));
+  return launch_norm<__nv_bfloat16>(g, vec, as_stream(stream));
 }
 
 }  // extern "C"
