@@ -32,17 +32,53 @@ struct Vec {
   static constexpr int kLanes = kFp8Group / kV;
 };
 
-__device__ __forceinline__ float to_f32(float v) { return v; }
-__device__ __forceinline__ float to_f32(__half v) { return __half2float(v); }
-__device__ __forceinline__ float to_f32(__nv_bfloat16 v) { return __bfloat162float(v); }
+// A 16-byte piece as f32 values, and back with one rounding.
+__device__ __forceinline__ void unpack(const uint4& p, float (&v)[4], const float*) {
+  v[0] = __uint_as_float(p.x); v[1] = __uint_as_float(p.y);
+  v[2] = __uint_as_float(p.z); v[3] = __uint_as_float(p.w);
+}
+__device__ __forceinline__ void unpack(const uint4& p, float (&v)[8], const __half*) {
+  const uint32_t w[4] = {p.x, p.y, p.z, p.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+    v[2 * i] = f.x;
+    v[2 * i + 1] = f.y;
+  }
+}
+__device__ __forceinline__ void unpack(const uint4& p, float (&v)[8], const __nv_bfloat16*) {
+  const uint32_t w[4] = {p.x, p.y, p.z, p.w};
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    v[2 * i] = __uint_as_float(w[i] << 16);
+    v[2 * i + 1] = __uint_as_float(w[i] & 0xFFFF0000u);
+  }
+}
 template <typename T>
-__device__ __forceinline__ T from_f32(float v);
-template <>
-__device__ __forceinline__ float from_f32<float>(float v) { return v; }
-template <>
-__device__ __forceinline__ __half from_f32<__half>(float v) { return __float2half_rn(v); }
-template <>
-__device__ __forceinline__ __nv_bfloat16 from_f32<__nv_bfloat16>(float v) { return __float2bfloat16_rn(v); }
+__device__ __forceinline__ void unpack(const uint4& p, float (&v)[Vec<T>::kV]) {
+  unpack(p, v, static_cast<const T*>(nullptr));
+}
+__device__ __forceinline__ uint4 pack(const float (&v)[4], const float*) {
+  return make_uint4(__float_as_uint(v[0]), __float_as_uint(v[1]), __float_as_uint(v[2]), __float_as_uint(v[3]));
+}
+__device__ __forceinline__ uint4 pack(const float (&v)[8], const __half*) {
+  uint32_t w[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const __half2 h = __floats2half2_rn(v[2 * i], v[2 * i + 1]);
+    w[i] = *reinterpret_cast<const uint32_t*>(&h);
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
+__device__ __forceinline__ uint4 pack(const float (&v)[8], const __nv_bfloat16*) {
+  uint32_t w[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) {
+    const __nv_bfloat162 h = __floats2bfloat162_rn(v[2 * i], v[2 * i + 1]);
+    w[i] = *reinterpret_cast<const uint32_t*>(&h);
+  }
+  return make_uint4(w[0], w[1], w[2], w[3]);
+}
 
 // Columns [c, c + kV) of a row of k columns as its 16 bytes (zero past the row).
 // kVec: rows start at multiples of 16 bytes and k is a multiple of kV.
@@ -58,13 +94,6 @@ __device__ __forceinline__ uint4 load_piece(const T* row, int c, int k) {
   for (int i = 0; i < Vec<T>::kV; ++i)
     if (c + i < k) e[i] = row[c + i];
   return p;
-}
-
-template <typename T>
-__device__ __forceinline__ void unpack(const uint4& p, float (&v)[Vec<T>::kV]) {
-  const T* e = reinterpret_cast<const T*>(&p);
-#pragma unroll
-  for (int i = 0; i < Vec<T>::kV; ++i) v[i] = to_f32(e[i]);
 }
 
 // The group maximum of |z| (at least 2^-100) over the group's lanes.
@@ -117,15 +146,17 @@ struct RowArgs {
 
 constexpr int kRowThreads = 256;
 
-// One CTA per row and 256 * kN * kV columns: a thread requests its kN pieces of
+// One row and 256 * kN * kV columns per CTA, or kNarrow: blockDim.y rows of one piece
+// per thread (blockDim.x is a multiple of 32).  A thread requests its kN pieces of
 // every input before it uses the first.
-template <int kMode, typename T, bool kVec, int kN>
+template <int kMode, typename T, bool kVec, bool kNarrow, int kN>
 __global__ void __launch_bounds__(kRowThreads) k_fp8_rows(const RowArgs g) {
   constexpr int kV = Vec<T>::kV;
   pdl_launch_dependents();
   pdl_wait();
-  const int c0 = (int)(blockIdx.x * kN * kRowThreads + threadIdx.x) * kV;
-  for (int64_t row = blockIdx.y; row < g.m; row += gridDim.y) {
+  const int ty = kNarrow ? (int)blockDim.y : 1;
+  const int c0 = (kNarrow ? (int)threadIdx.x : (int)(blockIdx.x * kN * kRowThreads + threadIdx.x)) * kV;
+  for (int64_t row = (int64_t)blockIdx.y * ty + (kNarrow ? threadIdx.y : 0); row < g.m; row += (int64_t)gridDim.y * ty) {
     const T* arow = static_cast<const T*>(g.a) + row * g.lda;
     const T* brow = static_cast<const T*>(g.b) + row * g.ldb;
     uint4 pa[kN], pb[kMode == kRowSwiglu ? kN : 1];
@@ -221,7 +252,7 @@ __device__ __forceinline__ void norm_weights(const NormArgs& g, int c, float (&w
 
 // One row per threadIdx.y: blockDim.x threads take kN pieces each per sweep (one
 // sweep for most widths).  Several rows share a CTA only where a warp takes a row.
-template <typename T, bool kVec, int kN>
+template <typename T, bool kVec, bool kRes, int kN>
 __global__ void __launch_bounds__(kN == 1 ? 1024 : 512, kN == 1 ? 1 : 2) k_fp8_norm(const NormArgs g) {
   constexpr int kV = Vec<T>::kV;
   __shared__ float red[32];
@@ -230,36 +261,34 @@ __global__ void __launch_bounds__(kN == 1 ? 1024 : 512, kN == 1 ? 1 : 2) k_fp8_n
   const int64_t row = (int64_t)blockIdx.x * blockDim.y + threadIdx.y;
   if (row >= g.m) return;  // a whole warp: CTAs of one row have no such row
   const T* xrow = static_cast<const T*>(g.x) + row * g.ldx;
-  T* rrow = g.residual ? static_cast<T*>(g.residual) + row * g.ldr : nullptr;
+  T* rrow = static_cast<T*>(g.residual) + row * g.ldr;
   float* scales = g.scales + row * g.lds;
   const int sweep = (int)blockDim.x * kN * kV;
   float ss = 0.0f, gm[kN];
   for (int s = 0; s < g.k; s += sweep) {
-    uint4 px[kN], pr[kN];
+    uint4 px[kN], pr[kRes ? kN : 1];
 #pragma unroll
     for (int i = 0; i < kN; ++i) {
       const int c = s + (int)(i * blockDim.x + threadIdx.x) * kV;
       px[i] = load_piece<kVec>(xrow, c, g.k);
-      if (rrow) pr[i] = load_piece<kVec, T>(rrow, c, g.k);
+      if constexpr (kRes) pr[i] = load_piece<kVec, T>(rrow, c, g.k);
     }
 #pragma unroll
     for (int i = 0; i < kN; ++i) {
       const int c = s + (int)(i * blockDim.x + threadIdx.x) * kV;
       float h[kV], w[kV];
       unpack<T>(px[i], h);
-      if (rrow) {
+      if constexpr (kRes) {
         float r[kV];
         unpack<T>(pr[i], r);
-        uint4 p;
-        T* e = reinterpret_cast<T*>(&p);
 #pragma unroll
-        for (int j = 0; j < kV; ++j) {
-          e[j] = from_f32<T>(h[j] + r[j]);
-          h[j] = to_f32(e[j]);
-        }
+        for (int j = 0; j < kV; ++j) h[j] += r[j];
+        const uint4 p = pack(h, static_cast<const T*>(nullptr));
+        unpack<T>(p, h);
         if constexpr (kVec) {
           if (c < g.k) *reinterpret_cast<uint4*>(rrow + c) = p;
         } else {
+          const T* e = reinterpret_cast<const T*>(&p);
 #pragma unroll
           for (int j = 0; j < kV; ++j)
             if (c + j < g.k) rrow[c + j] = e[j];
@@ -321,13 +350,21 @@ bool vec_rows(const void* p, int64_t ld, uint32_t dtype) {
 
 template <int kMode, typename T>
 int launch_rows(const RowArgs& g, bool vec, cudaStream_t st) {
-  // two pieces per thread once that still leaves every SM four CTAs
+  // Narrow rows share a CTA; wide ones take two pieces per thread once that still
+  // leaves every SM four CTAs (16384 x 8192 bf16 SwiGLU: 104 us with two, 120 with one).
   const int64_t pieces = (g.k + Vec<T>::kV - 1) / Vec<T>::kV;
   vec = vec && g.k % Vec<T>::kV == 0;
+  if (pieces <= kRowThreads / 2) {
+    const unsigned tx = (unsigned)((pieces + 31) / 32 * 32), ty = kRowThreads / tx;
+    const dim3 grid(1, (unsigned)std::min<int64_t>((g.m + ty - 1) / ty, 65535));
+    return launch_pdl(vec ? k_fp8_rows<kMode, T, true, true, 1> : k_fp8_rows<kMode, T, false, true, 1>, grid,
+                      dim3(tx, ty), 0, st, g);
+  }
   const bool many = vec && g.m * ((pieces + 2 * kRowThreads - 1) / (2 * kRowThreads)) >= 4 * (int64_t)sm_count();
   const int64_t cols = (int64_t)kRowThreads * (many ? 2 : 1);
-  const dim3 grid((unsigned)((pieces + cols - 1) / cols), (unsigned)(g.m < 65535 ? g.m : 65535));
-  return launch_pdl(many ? k_fp8_rows<kMode, T, true, 2> : vec ? k_fp8_rows<kMode, T, true, 1> : k_fp8_rows<kMode, T, false, 1>,
+  const dim3 grid((unsigned)((pieces + cols - 1) / cols), (unsigned)std::min<int64_t>(g.m, 65535));
+  return launch_pdl(many ? k_fp8_rows<kMode, T, true, false, 2>
+                    : vec ? k_fp8_rows<kMode, T, true, false, 1> : k_fp8_rows<kMode, T, false, false, 1>,
                     grid, dim3(kRowThreads), 0, st, g);
 }
 
@@ -338,18 +375,29 @@ int dispatch_rows(const RowArgs& g, uint32_t dtype, bool vec, cudaStream_t st) {
   return launch_rows<kMode, __nv_bfloat16>(g, vec, st);
 }
 
-template <typename T>
+template <typename T, bool kRes>
 int launch_norm(const NormArgs& g, bool vec, cudaStream_t st) {
   // Few rows: one piece per thread, up to 1024 threads, for the latency of one
-  // round of loads.  Many rows: four pieces per thread (a warp per row where that
-  // covers it), for few threads per row and many rows in flight.
+  // round of loads.  Many rows: few threads per row and many pieces each, so that a
+  // row's sum costs little and many rows are in flight (16384 x 8192 bf16 with a
+  // residual: 151 us with four pieces, 190 with two, 321 with one); without the
+  // residual's registers, eight.
+  constexpr int kMany = kRes ? 4 : 8;
   const int64_t pieces = (g.k + Vec<T>::kV - 1) / Vec<T>::kV;
   vec = vec && g.k % Vec<T>::kV == 0;
-  const int n = g.m > 2 * (int64_t)sm_count() && vec ? 4 : 1;
+  const bool many = g.m > 2 * (int64_t)sm_count();
+  const int n = !many || !vec ? 1 : pieces <= 64 ? 2 : kMany;
   const unsigned tx = (unsigned)std::min<int64_t>(n == 1 ? 1024 : 512, ((pieces + n - 1) / n + 31) / 32 * 32);
   const unsigned ty = tx == 32 ? 8 : 1;
-  return launch_pdl(n == 4 ? k_fp8_norm<T, true, 4> : vec ? k_fp8_norm<T, true, 1> : k_fp8_norm<T, false, 1>,
+  return launch_pdl(n == kMany ? k_fp8_norm<T, true, kRes, kMany>
+                    : n == 2 ? k_fp8_norm<T, true, kRes, 2>
+                    : vec ? k_fp8_norm<T, true, kRes, 1> : k_fp8_norm<T, false, kRes, 1>,
                     dim3((unsigned)((g.m + ty - 1) / ty)), dim3(tx, ty), 0, st, g);
+}
+
+template <typename T>
+int dispatch_norm(const NormArgs& g, bool vec, cudaStream_t st) {
+  return g.residual ? launch_norm<T, true>(g, vec, st) : launch_norm<T, false>(g, vec, st);
 }
 
 }  // namespace
@@ -390,9 +438,9 @@ int ah_fp8_add_rms_norm(const void* x, int64_t ldx, void* residual, int64_t ldr,
   AH_REQUIRE(eps >= 0.0f, "fp8_add_rms_norm: eps must be >= 0");
   const NormArgs g{x, residual, norm_w, ldx, ldr, m, (int)k, q, ldq, scales, lds, norm_dtype, eps};
   const bool vec = vec_rows(x, ldx, dtype) && (!residual || vec_rows(residual, ldr, dtype)) && aligned16(norm_w);
-  if (dtype == AH_DTYPE_F32) return launch_norm<float>(g, vec, as_stream(stream));
-  if (dtype == AH_DTYPE_F16) return launch_norm<__half>(g, vec, as_stream(stream));
-  return launch_norm<__nv_bfloat16>(g, vec, as_stream(stream));
+  if (dtype == AH_DTYPE_F32) return dispatch_norm<float>(g, vec, as_stream(stream));
+  if (dtype == AH_DTYPE_F16) return dispatch_norm<__half>(g, vec, as_stream(stream));
+  return dispatch_norm<__nv_bfloat16>(g, vec, as_stream(stream));
 }
 
 }  // extern "C"
