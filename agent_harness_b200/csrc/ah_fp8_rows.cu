@@ -386,13 +386,14 @@ int launch_norm(const NormArgs& g, bool vec, cudaStream_t st) {
   const int64_t pieces = (g.k + Vec<T>::kV - 1) / Vec<T>::kV;
   vec = vec && g.k % Vec<T>::kV == 0;
   const bool many = g.m > 2 * (int64_t)sm_count();
-  const int n = !many || !vec ? 1 : pieces <= 64 ? 2 : kMany;
+  const int n = !many ? 1 : pieces <= (vec ? 64 : 256) ? 2 : kMany;
   const unsigned tx = (unsigned)std::min<int64_t>(n == 1 ? 1024 : 512, ((pieces + n - 1) / n + 31) / 32 * 32);
   const unsigned ty = tx == 32 ? 8 : 1;
-  return launch_pdl(n == kMany ? k_fp8_norm<T, true, kRes, kMany>
-                    : n == 2 ? k_fp8_norm<T, true, kRes, 2>
-                    : vec ? k_fp8_norm<T, true, kRes, 1> : k_fp8_norm<T, false, kRes, 1>,
-                    dim3((unsigned)((g.m + ty - 1) / ty)), dim3(tx, ty), 0, st, g);
+  auto kernel = vec ? (n == 1 ? k_fp8_norm<T, true, kRes, 1>
+                       : n == 2 ? k_fp8_norm<T, true, kRes, 2> : k_fp8_norm<T, true, kRes, kMany>)
+                    : (n == 1 ? k_fp8_norm<T, false, kRes, 1>
+                       : n == 2 ? k_fp8_norm<T, false, kRes, 2> : k_fp8_norm<T, false, kRes, kMany>);
+  return launch_pdl(kernel, dim3((unsigned)((g.m + ty - 1) / ty)), dim3(tx, ty), 0, st, g);
 }
 
 template <typename T>
