@@ -124,7 +124,8 @@ SIGNATURES = {
     "ah_fp8w_destroy": (i32, [vp]),
     "ah_fp8w_shape": (i32, [vp, C.POINTER(i64), C.POINTER(i64)]),
     "ah_fp8w_weight_bytes": (i64, [vp]),
-    "ah_fp8w_matmul": (i32, [vp, vp, i64, vp, i64, i64, vp, i64, u32, vp]),
+    "ah_fp8w_matmul_workspace_bytes": (i32, [vp, i64, C.POINTER(sz)]),
+    "ah_fp8w_matmul": (i32, [vp, vp, i64, vp, i64, i64, vp, i64, u32, vp, sz, vp]),
     "ah_fp8_ffn_workspace_bytes": (i32, [vp, vp, i64, C.POINTER(sz)]),
     "ah_fp8_ffn": (i32, [vp, vp, vp, i64, vp, i64, u32, vp, u32, f32, i64, vp, i64, u32, vp, sz, vp]),
     "ah_host_gemv_4bit_into": (i32, [vp, vp, vp, vp, sz, sz, sz]),

@@ -6,6 +6,7 @@
 // b runs over the blocks of 128 columns.  The inner sums are exact products
 // summed in f32; the scales multiply each block's sum in f32.
 #include <algorithm>
+#include <climits>
 #include <mutex>
 #include <new>
 
@@ -595,10 +596,7 @@ int launch_small(SmallArgs& p, cudaStream_t st) {
 
 template <bool kGlu>
 int dispatch_small(SmallArgs& p, cudaStream_t st) {
-  if (p.g.m <= 16) return launch_small<16, kGlu>(p, st);
-  if (p.g.m <= 32) return launch_small<32, kGlu>(p, st);
-  if (kGlu || p.g.m <= 64) return launch_small<64, kGlu>(p, st);
-  if constexpr (!kGlu) return launch_small<128, false>(p, st);
+  return p.g.m <= 16 ? launch_small<16, kGlu>(p, st) : p.g.m <= 32 ? launch_small<32, kGlu>(p, st) : launch_small<64, kGlu>(p, st);
 }
 
 // ---- many tokens: CTA pairs, 256 tokens x 256 weight rows ---------------------------------
@@ -619,8 +617,8 @@ int dispatch_small(SmallArgs& p, cudaStream_t st) {
 constexpr int kBigStages = 6;
 constexpr int kBigThreads = 384;
 // Registers: 384 threads start with 168 each (64512); the first four warps drop
-// to 40 and the eight readers rise to 232 (128 * 40 + 256 * 232 = 64512).
-constexpr int kBigRegsFew = 40, kBigRegsMany = 232;
+// to 24 and the eight readers rise to 240 (128 * 24 + 256 * 240 = 64512).
+constexpr int kBigRegsFew = 24, kBigRegsMany = 240;
 constexpr int kBigTokens = 256;
 
 struct Big {
@@ -634,12 +632,49 @@ struct Big {
   static_assert(kDynamic <= 227 * 1024, "one CTA per SM");
 };
 
+// How the tiles are dealt out.  Tiles [0, whole) go round robin to the pairs of the
+// grid, each over all column blocks.  Each of the `rest` tiles, fewer than a full
+// round, is cut along the column blocks into `parts` pieces for as many pairs: pair
+// p's sums go to partial slot p as f32 [256 columns][256 tokens], and k_fp8_join adds
+// a tile's slots in K order.
+struct BigSplit {
+  int whole, rest, parts;
+};
+
+// The tiles of one pair, in order: tile, column blocks [b0, b1), partial slot (or
+// -1: the whole tile).  What does not change stays in the kernel's arguments.
+struct BigWalk {
+  int tile, b0, b1, slot, at;
+  __device__ __forceinline__ BigWalk() : at((int)blockIdx.x / 2) {}
+  __device__ __forceinline__ bool next(const BigSplit& s, int kb) {
+    b0 = 0;
+    b1 = kb;
+    slot = -1;
+    tile = at;
+    if (at < s.whole) {
+      at += (int)gridDim.x / 2;
+      return true;
+    }
+    const int pair = (int)blockIdx.x / 2;
+    if (at == INT_MAX || pair >= s.rest * s.parts) return false;
+    at = INT_MAX;
+    const int piece = pair % s.parts;
+    tile = s.whole + pair / s.parts;
+    b0 = (int)((int64_t)kb * piece / s.parts);
+    b1 = (int)((int64_t)kb * (piece + 1) / s.parts);
+    slot = pair;
+    return true;
+  }
+};
+
 struct BigArgs {
   CUtensorMap tm_a;  // e4m3 activations [m][cols], box 128 x 128, 128-byte swizzle
   CUtensorMap tm_w;  // weight images as bytes [images * 128][128], box 128 x 128
   CUtensorMap tm_y;  // y [m][rows], box 128 bytes x 32 rows, 128-byte swizzle (when y_map)
   MatmulArgs g;
   bool y_map;
+  BigSplit split;
+  float* partial;
   uint8_t* act_q;
   int64_t ld_act;
   float* act_scales;
@@ -687,7 +722,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kBigThreads, 1) k_fp
   const int warp = warp_index(), lane = threadIdx.x & 31;
   const int rank = (int)cluster_ctarank();
   const int mt = (int)((g.m + kBigTokens - 1) / kBigTokens), nt = (int)g.nt, kb = (int)g.kb;
-  const int tiles = mt * ((nt + 1) / 2), first = blockIdx.x / 2, step = gridDim.x / 2;
+  BigWalk walk;
 
   if (threadIdx.x == 0) {
     for (int i = 0; i < kBigStages; ++i) {
@@ -723,15 +758,16 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kBigThreads, 1) k_fp
         tma_load_2d_pair(st0 + s * Big::kStageBytes + kFp8TileBytes, &p.tm_w, 0,
                          (int)fp8_image(g.gate_up, kb, t, b) * kFp8Group, full0 + s * 8);
       };
-      int left = min(kb, kBigStages);  // blocks whose weights are under way
+      bool more = walk.next(p.split, kb);
+      int left = more ? min(walk.b1 - walk.b0, kBigStages) : 0;  // blocks whose weights are under way
       if (elected)
-        for (int i = 0; i < left; ++i) weights(i, first / mt, i);
+        for (int i = 0; i < left; ++i) weights(i, walk.tile / mt, walk.b0 + i);
       pdl_wait();  // the tokens come from the preceding grid
       int s = 0;
       uint32_t ph = 1;  // the stages start empty
-      for (int tile = first; tile < tiles; tile += step) {
-        const int unit = tile / mt, row = tile % mt * kBigTokens + rank * 128;
-        for (int b = 0; b < kb; ++b) {
+      for (; more; more = walk.next(p.split, kb)) {
+        const int unit = walk.tile / mt, row = walk.tile % mt * kBigTokens + rank * 128;
+        for (int b = walk.b0; b < walk.b1; ++b) {
           wait_bar(&empty[s], ph, p.err, abort_flag);
           if (elected) {
             if (left <= 0) weights(s, unit, b);
@@ -752,8 +788,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kBigThreads, 1) k_fp
       constexpr uint32_t idesc = idesc_e4m3(256, 256);
       int s = 0, buf = 0;
       uint32_t ph = 0, dph = 1;  // the buffers start empty
-      for (int tile = first; tile < tiles; tile += step)
-        for (int b = 0; b < kb; ++b) {
+      while (walk.next(p.split, kb))
+        for (int b = walk.b0; b < walk.b1; ++b) {
           wait_bar(&full[s], ph, p.err, abort_flag);
           wait_bar(&d_empty[buf], dph, p.err, abort_flag);
           tc_fence_after();
@@ -783,13 +819,15 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kBigThreads, 1) k_fp
     const uint32_t d_empty0 = mapa_shared(smem_u32(d_empty), 0);
     const uint32_t lane_addr = tmem + ((uint32_t)(q * 32) << 16) + h * 64;
     const bool vec = (reinterpret_cast<uintptr_t>(g.ascales) & 15) == 0 && g.lds % 4 == 0;
-    const bool wvec = kb % 4 == 0;
+    const bool wvec = kb % 4 == 0;  // rows of scales start at multiples of 16 bytes
     uint8_t* stage = smem + Big::kStage + (warp - 4) * 4096;
     pdl_wait();  // the scales come from the preceding grid
     int buf = 0;
     uint32_t ph = 0;
-    for (int tile = first; tile < tiles; tile += step) {
-      const int unit = tile / mt, m0 = tile % mt * kBigTokens + rank * 128 + q * 32;
+    while (walk.next(p.split, kb)) {
+      const int unit = walk.tile / mt, m0 = walk.tile % mt * kBigTokens + rank * 128 + q * 32;
+      const int b0 = walk.b0, b1 = walk.b1;
+      const bool va = vec && b0 % 4 == 0, vw = wvec && b0 % 4 == 0;
       const int64_t tok = m0 + lane;
       const float* arow = g.ascales + (tok < g.m ? tok : 0) * g.lds;  // past m: stored nowhere
       const float* w0 = g.wscales + (int64_t)(unit * 2) * kb;
@@ -798,20 +836,20 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kBigThreads, 1) k_fp
 #pragma unroll
       for (int j = 0; j < 64; ++j) acc[0][j] = acc[1][j] = 0.0f;
       float a4[4];
-      load_scales4(arow, 0, kb, vec, a4);
-      for (int b4 = 0; b4 < kb; b4 += 4) {
+      load_scales4(arow, b0, b1, va, a4);
+      for (int b4 = b0; b4 < b1; b4 += 4) {
         float s0[4], s1[4];
-        load_scales4(w0, b4, kb, wvec, s0);
-        load_scales4(w1, b4, kb, wvec, s1);
+        load_scales4(w0, b4, b1, vw, s0);
+        load_scales4(w1, b4, b1, vw, s1);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
           s0[i] *= a4[i];
           s1[i] *= a4[i];
         }
-        load_scales4(arow, b4 + 4, kb, vec, a4);
+        load_scales4(arow, b4 + 4, b1, va, a4);
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-          if (b4 + i >= kb) break;
+          if (b4 + i >= b1) break;
           wait_bar(&d_full[buf], ph, p.err, abort_flag);
           tc_fence_after();
           const uint32_t ta = lane_addr + buf * 256;
@@ -839,6 +877,17 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kBigThreads, 1) k_fp
         }
       }
       const bool ok = !__any_sync(0xFFFFFFFFu, *abort_flag);  // after a give-up nothing is stored
+      if (walk.slot >= 0) {
+        // columns 64 h + j of weight tile t at 128 t + 64 h + j: a warp stores 32 tokens
+        float* out = p.partial + ((int64_t)walk.slot * 256 + h * 64) * kBigTokens + rank * 128 + q * 32 + lane;
+        if (ok && tok < g.m) {
+#pragma unroll
+          for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int j = 0; j < 64; ++j) out[(t * 128 + j) * kBigTokens] = acc[t][j];
+        }
+        continue;
+      }
       if constexpr (kGlu) {
         const int64_t n_ff = g.rows / 2, c0 = (int64_t)unit * kFp8Group + h * 64;
         float fm = kFp8Tiny;
@@ -911,15 +960,30 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kBigThreads, 1) k_fp
             bulk_commit();
           }
         }
-      } else if (tok < g.m) {
+      } else {
+        // y that no tensor map can address: 32 x 32 f32 boxes through the warp's
+        // stage, each token's 32 columns written by the whole warp
         const int64_t rows = g.gate_up ? g.rows / 2 : g.rows;  // rows of a tile's source
+        float* box = reinterpret_cast<float*>(stage);
 #pragma unroll
-        for (int c = 0; c < 2; ++c) {
-          const int64_t r0 = (int64_t)(g.gate_up ? unit : unit * 2 + c) * kFp8Group + h * 64;
-          const int64_t base = tok * g.ldy + (g.gate_up ? c * rows : 0) + r0;
+        for (int c = 0; c < 4; ++c) {
+          __syncwarp();
 #pragma unroll
-          for (int j = 0; j < 64; ++j)
-            if (r0 + j < rows) store_y(g.y, base + j, g.y_dtype, acc[c][j]);
+          for (int j = 0; j < 32; ++j) box[lane * 32 + (j ^ lane)] = acc[c / 2][c % 2 * 32 + j];
+          __syncwarp();
+          const int64_t r = (int64_t)(g.gate_up ? unit : unit * 2 + c / 2) * kFp8Group + h * 64 + c % 2 * 32 + lane;
+          if (r < rows) {
+            const int64_t at = (g.gate_up ? c / 2 * rows : 0) + r;
+            const int live = (int)min((int64_t)32, g.m - m0);
+            auto write = [&](auto* y, auto convert) {
+              y += (int64_t)m0 * g.ldy + at;
+#pragma unroll 8
+              for (int i = 0; i < live; ++i, y += g.ldy) *y = convert(box[i * 32 + (lane ^ i)]);
+            };
+            if (g.y_dtype == AH_DTYPE_F32) write(static_cast<float*>(g.y), [](float v) { return v; });
+            else if (g.y_dtype == AH_DTYPE_F16) write(static_cast<__half*>(g.y), [](float v) { return __float2half_rn(v); });
+            else write(static_cast<__nv_bfloat16*>(g.y), [](float v) { return __float2bfloat16_rn(v); });
+          }
         }
       }
     }
@@ -936,8 +1000,110 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kBigThreads, 1) k_fp
   }
 }
 
+// Joins one split tile's partial sums for 32 tokens (x: chunk of tokens, y: tile of
+// the rest): 32 warps of eight columns, lanes over the tokens.
+constexpr int kJoinThreads = 1024;
 template <bool kGlu>
-int launch_big(BigArgs& p, cudaStream_t st) {
+__global__ void __launch_bounds__(kJoinThreads) k_fp8_join(const __grid_constant__ BigArgs p) {
+  __shared__ float tr[kGlu ? 1 : 32][256 + 1];  // [token][column]
+  __shared__ uint32_t maxima[kGlu ? 32 * 32 : 1];
+  pdl_launch_dependents();
+  const MatmulArgs& g = p.g;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int mt = (int)((g.m + kBigTokens - 1) / kBigTokens), parts = p.split.parts;
+  const int r = blockIdx.y, tile = p.split.whole + r, unit = tile / mt;
+  const int64_t m0 = (int64_t)(tile % mt) * kBigTokens + blockIdx.x * 32, tok = m0 + lane;
+  if (m0 >= g.m) return;
+  // this warp's columns: SwiGLU, four gate columns and the same four up columns
+  const int c0 = kGlu ? warp * 4 : warp * 8;
+  auto column = [&](int j) { return kGlu ? j / 4 * 128 + c0 + j % 4 : c0 + j; };
+  const float* in = p.partial + (int64_t)r * parts * 256 * kBigTokens + blockIdx.x * 32 + lane;
+  float acc[8];
+#pragma unroll
+  for (int j = 0; j < 8; ++j) acc[j] = 0.0f;
+  pdl_wait();
+  if (tok < g.m) {
+    for (int q = 0; q < parts; q += 4) {  // four pieces' loads in flight
+      float v[4][8];
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[i][j] = q + i < parts ? in[((q + i) * 256 + column(j)) * kBigTokens] : 0.0f;
+#pragma unroll
+      for (int i = 0; i < 4; ++i)
+#pragma unroll
+        for (int j = 0; j < 8; ++j) acc[j] += v[i][j];
+    }
+  }
+  if constexpr (kGlu) {
+    const int64_t n_ff = g.rows / 2, col = (int64_t)unit * kFp8Group + c0;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) acc[j] = fp8_silu_mul(acc[j], acc[j + 4]);
+    maxima[warp * 32 + lane] = __float_as_uint(max_abs3(max_abs3(kFp8Tiny, acc[0], acc[1]), acc[2], acc[3]));
+    __syncthreads();
+    uint32_t mx = 0;  // a NaN's bits are above every number's
+#pragma unroll
+    for (int i = 0; i < 32; ++i) mx = max(mx, maxima[i * 32 + lane]);
+    const float gm = __uint_as_float(mx), inv = fp8_inverse(gm);
+    if (tok < g.m) {
+      const uint32_t w = cvt_e4m3x4(acc[0] * inv, acc[1] * inv, acc[2] * inv, acc[3] * inv);
+      uint8_t* qrow = p.act_q + tok * p.ld_act + col;  // ld_act is a multiple of 16
+      if (col + 4 <= n_ff) *reinterpret_cast<uint32_t*>(qrow) = w;
+      else
+        for (int i = 0; i < 4 && col + i < n_ff; ++i) qrow[i] = (uint8_t)(w >> (8 * i));
+      if (warp == 0) p.act_scales[tok * p.lds_act + unit] = gm * (1.0f / kFp8Max);
+    }
+  } else {
+#pragma unroll
+    for (int j = 0; j < 8; ++j) tr[lane][c0 + j] = acc[j];
+    __syncthreads();
+    // warp w writes token w's 256 columns
+    const int64_t rows = g.gate_up ? g.rows / 2 : g.rows;
+    if (m0 + warp < g.m) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        const int t = i / 4;  // weight tile of the pair
+        const int64_t row = (int64_t)(g.gate_up ? unit : unit * 2 + t) * kFp8Group + i % 4 * 32 + lane;
+        if (row < rows)
+          store_y(g.y, (m0 + warp) * g.ldy + (g.gate_up ? t * rows : 0) + row, g.y_dtype, tr[warp][i * 32 + lane]);
+      }
+    }
+  }
+}
+
+int check_device(const char* who, const AhFp8Weight* w) {
+  int dev = -1;
+  AH_CUDA_TRY(cudaGetDevice(&dev));
+  AH_REQUIRE(dev == w->device, "%s: the weight lives on device %d, device %d is current", who, w->device, dev);
+  return AH_OK;
+}
+
+// The pairs of a launch and how its tiles are dealt out.  Splitting the tiles past
+// the last full round saves column blocks' time (about 0.45 us each) and costs a
+// launch (3 us) and the partial sums' way to L2 and back (about 6 TB/s).
+struct BigPlan {
+  int pairs;
+  BigSplit split;
+  size_t bytes;  // partial sums
+};
+
+BigPlan big_plan(const AhFp8Weight* w, int64_t m) {
+  const int64_t tiles = (m + kBigTokens - 1) / kBigTokens * ((w->nt + 1) / 2), pairs = std::max(1, sm_count() / 2);
+  const int64_t rest = tiles % pairs, kb = w->kb;
+  BigPlan p{(int)std::min(tiles, pairs), {(int)tiles, 0, 0}, 0};
+  const int64_t parts = rest ? std::min<int64_t>(pairs / rest, kb / 2) : 0;  // two column blocks each at least
+  if (parts < 2) return p;
+  const double saved = 0.45e-6 * (double)(kb - (kb + parts - 1) / parts);
+  const double moved = 2.0 * (double)(rest * parts) * (double)std::min<int64_t>(m, kBigTokens) * 256 * sizeof(float);
+  if (saved < 3e-6 + moved / 6e12) return p;
+  p.pairs = (int)(tiles > pairs ? pairs : rest * parts);
+  p.split = BigSplit{(int)(tiles - rest), (int)rest, (int)parts};
+  p.bytes = (size_t)(rest * parts) * 256 * kBigTokens * sizeof(float);
+  return p;
+}
+
+template <bool kGlu>
+int launch_big(BigArgs& p, const BigPlan& plan, cudaStream_t st) {
   const MatmulArgs& g = p.g;
   int rc = encode_rows(&p.tm_a, g.a, (uint64_t)g.cols, (uint64_t)g.m, (uint64_t)g.lda, 128);
   if (rc != AH_OK) return rc;
@@ -965,26 +1131,56 @@ int launch_big(BigArgs& p, cudaStream_t st) {
     attr[dev] = cudaFuncSetAttribute(k_fp8_big<kGlu>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Big::kDynamic);
   });
   AH_CUDA_TRY(attr[dev]);
-  const int64_t tiles = (g.m + kBigTokens - 1) / kBigTokens * ((g.nt + 1) / 2);
-  AH_REQUIRE(tiles < (1 << 30) && g.nt * g.kb < (1 << 24) && g.m <= 0x7FFFFF00,
-             "fp8w_matmul: too many tiles for one launch");
-  return launch_pdl(k_fp8_big<kGlu>, dim3((unsigned)(2 * std::min<int64_t>(tiles, sm_count() / 2))), dim3(kBigThreads),
-                    Big::kDynamic, st, (const BigArgs)p);
+  p.split = plan.split;
+  rc = launch_pdl(k_fp8_big<kGlu>, dim3((unsigned)(2 * plan.pairs)), dim3(kBigThreads), Big::kDynamic, st,
+                  (const BigArgs)p);
+  if (rc != AH_OK || plan.split.rest == 0) return rc;
+  const unsigned chunks = (unsigned)std::min<int64_t>(kBigTokens / 32, (g.m + 31) / 32);
+  return launch_pdl(k_fp8_join<kGlu>, dim3(chunks, (unsigned)plan.split.rest), dim3(kJoinThreads), 0, st, (const BigArgs)p);
 }
 
-bool use_big(int64_t m) { return m > 128; }
+bool use_big(int64_t m) { return m > 64; }
 
-int check_device(const char* who, const AhFp8Weight* w) {
-  int dev = -1;
-  AH_CUDA_TRY(cudaGetDevice(&dev));
-  AH_REQUIRE(dev == w->device, "%s: the weight lives on device %d, device %d is current", who, w->device, dev);
+// Bytes of partial sums a product of m rows uses.
+size_t matmul_bytes(const AhFp8Weight* w, int64_t m) { return m > 0 && use_big(m) ? big_plan(w, m).bytes : 0; }
+
+int check_matmul(const AhFp8Weight* w, int64_t m) {
+  AH_REQUIRE(w, "fp8w_matmul: null weight");
+  AH_REQUIRE(m >= 0 && m <= 0x7FFFFF00, "fp8w_matmul: m must be 0 .. 2^31 - 256");
+  AH_REQUIRE((m + kBigTokens - 1) / kBigTokens * ((w->nt + 1) / 2) < (1 << 30) && w->nt * w->kb < (1 << 24),
+             "fp8w_matmul: too many tiles for one launch");
   return AH_OK;
 }
 
+// The rest of a product's launch, for y or for SwiGLU's outputs (set in p by `set`).
+template <bool kGlu, typename Set>
+int run_matmul(const MatmulArgs& g, const AhFp8Weight* w, float* partial, size_t bytes, cudaStream_t st, Set set) {
+  if (use_big(g.m)) {
+    BigPlan plan = big_plan(w, g.m);
+    AH_REQUIRE(!partial || bytes >= plan.bytes, "fp8w_matmul: workspace of %zu bytes, %zu needed", bytes, plan.bytes);
+    if (plan.split.rest && !partial) {  // no workspace: no split
+      const int64_t tiles = plan.split.whole + plan.split.rest;
+      plan.pairs = (int)std::min<int64_t>(tiles, std::max(1, sm_count() / 2));
+      plan.split = BigSplit{(int)tiles, 0, 0};
+    }
+    BigArgs p{};
+    p.g = g;
+    p.partial = partial;
+    p.err = device_error_word();
+    set(p);
+    return launch_big<kGlu>(p, plan, st);
+  }
+  SmallArgs p{};
+  p.g = g;
+  p.err = device_error_word();
+  set(p);
+  return dispatch_small<kGlu>(p, st);
+}
+
 int matmul(const AhFp8Weight* w, const uint8_t* q, int64_t ldq, const float* scales, int64_t lds, int64_t m, void* y,
-           int64_t ldy, uint32_t y_dtype, cudaStream_t st) {
-  AH_REQUIRE(w, "fp8w_matmul: null weight");
-  AH_REQUIRE(m >= 0 && m <= 0x7FFFFFFF, "fp8w_matmul: m must be 0 .. 2^31 - 1");
+           int64_t ldy, uint32_t y_dtype, void* workspace, size_t bytes, cudaStream_t st) {
+  int rc = check_matmul(w, m);
+  if (rc != AH_OK) return rc;
   AH_REQUIRE(y_dtype == AH_DTYPE_F32 || y_dtype == AH_DTYPE_F16 || y_dtype == AH_DTYPE_BF16,
              "fp8w_matmul: output dtype %u is not f32, f16 or bf16", y_dtype);
   if (m == 0) return AH_OK;
@@ -992,43 +1188,34 @@ int matmul(const AhFp8Weight* w, const uint8_t* q, int64_t ldq, const float* sca
   AH_REQUIRE(aligned16(q) && ldq % 16 == 0 && ldq >= w->cols,
              "fp8w_matmul: q rows must start at multiples of 16 bytes, ldq >= cols");
   AH_REQUIRE(lds >= w->kb && ldy >= w->rows, "fp8w_matmul: lds below ceil(cols / 128) or ldy below rows");
-  const int rc = check_device("fp8w_matmul", w);
+  AH_REQUIRE(aligned16(workspace), "fp8w_matmul: the workspace must be 16-byte aligned");
+  rc = check_device("fp8w_matmul", w);
   if (rc != AH_OK) return rc;
   const MatmulArgs g{w->tiles, w->scales, w->rows, w->cols, w->nt, w->kb, w->gate_up, q, ldq, scales, lds, m, y, ldy,
                      y_dtype};
-  if (use_big(m)) {
-    BigArgs p{};
-    p.g = g;
-    p.err = device_error_word();
-    return launch_big<false>(p, st);
-  }
-  SmallArgs p{};
-  p.g = g;
-  p.err = device_error_word();
-  return dispatch_small<false>(p, st);
+  return run_matmul<false>(g, w, static_cast<float*>(workspace), bytes, st, [](auto&) {});
 }
 
 // silu(gate) * up of the products with a gate/up weight, quantised from f32.
 int matmul_swiglu(const AhFp8Weight* w, const uint8_t* q, int64_t ldq, const float* scales, int64_t lds, int64_t m,
-                  uint8_t* act_q, int64_t ld_act, float* act_scales, int64_t lds_act, cudaStream_t st) {
-  auto run = [&](auto p, auto launch) {
-    p.g = MatmulArgs{w->tiles, w->scales, w->rows, w->cols, w->nt, w->kb, true, q, ldq, scales, lds, m, nullptr, 0, 0};
+                  uint8_t* act_q, int64_t ld_act, float* act_scales, int64_t lds_act, float* partial, size_t bytes,
+                  cudaStream_t st) {
+  const MatmulArgs g{w->tiles, w->scales, w->rows, w->cols, w->nt, w->kb, true, q, ldq, scales, lds, m, nullptr, 0, 0};
+  return run_matmul<true>(g, w, partial, bytes, st, [&](auto& p) {
     p.act_q = act_q;
     p.ld_act = ld_act;
     p.act_scales = act_scales;
     p.lds_act = lds_act;
-    p.err = device_error_word();
-    return launch(p, st);
-  };
-  return use_big(m) ? run(BigArgs{}, launch_big<true>) : run(SmallArgs{}, dispatch_small<true>);
+  });
 }
 
 // ---- the feed-forward block ----------------------------------------------------------
 
-// Workspace: the norm's q and scales, the activation's q and scales.
+// Workspace: the norm's q and scales, the activation's q and scales, the products'
+// partial sums.
 struct FfnLayout {
   int64_t ldq1, lds1, ldq2, lds2;
-  size_t q1, s1, q2, s2, total;
+  size_t q1, s1, q2, s2, partial, partial_bytes, total;
 };
 
 FfnLayout ffn_layout(const AhFp8Weight* gu, const AhFp8Weight* down, int64_t m) {
@@ -1042,7 +1229,9 @@ FfnLayout ffn_layout(const AhFp8Weight* gu, const AhFp8Weight* down, int64_t m) 
   l.s1 = l.q1 + up((size_t)m * l.ldq1);
   l.q2 = l.s1 + up((size_t)m * l.lds1 * 4);
   l.s2 = l.q2 + up((size_t)m * l.ldq2);
-  l.total = l.s2 + up((size_t)m * l.lds2 * 4);
+  l.partial = l.s2 + up((size_t)m * l.lds2 * 4);
+  l.partial_bytes = std::max(matmul_bytes(gu, m), matmul_bytes(down, m));
+  l.total = l.partial + l.partial_bytes;
   return l;
 }
 
@@ -1050,8 +1239,8 @@ int check_ffn(const AhFp8Weight* gate_up, const AhFp8Weight* down, int64_t m) {
   AH_REQUIRE(gate_up && down, "fp8_ffn: null weight");
   AH_REQUIRE(gate_up->gate_up && !down->gate_up && down->cols == gate_up->rows / 2 && down->rows == gate_up->cols,
              "fp8_ffn: needs a gate/up weight of 2 * n_ff rows and a down weight [n_embd][n_ff]");
-  AH_REQUIRE(m >= 0 && m <= 0x7FFFFFFF, "fp8_ffn: m must be 0 .. 2^31 - 1");
-  return AH_OK;
+  const int rc = check_matmul(gate_up, m);
+  return rc != AH_OK ? rc : check_matmul(down, m);
 }
 
 
@@ -1104,9 +1293,17 @@ int64_t ah_fp8w_weight_bytes(const AhFp8Weight* w) {
   return w->rows * w->cols + w->nt * w->kb * 4;
 }
 
+int ah_fp8w_matmul_workspace_bytes(const AhFp8Weight* w, int64_t m, size_t* bytes) {
+  const int rc = check_matmul(w, m);
+  if (rc != AH_OK) return rc;
+  AH_REQUIRE(bytes, "fp8w_matmul_workspace_bytes: null output");
+  *bytes = matmul_bytes(w, m);
+  return AH_OK;
+}
+
 int ah_fp8w_matmul(const AhFp8Weight* w, const uint8_t* q, int64_t ldq, const float* scales, int64_t lds, int64_t m,
-                   void* y, int64_t ldy, uint32_t y_dtype, void* stream) {
-  return matmul(w, q, ldq, scales, lds, m, y, ldy, y_dtype, as_stream(stream));
+                   void* y, int64_t ldy, uint32_t y_dtype, void* workspace, size_t workspace_bytes, void* stream) {
+  return matmul(w, q, ldq, scales, lds, m, y, ldy, y_dtype, workspace, workspace_bytes, as_stream(stream));
 }
 
 int ah_fp8_ffn_workspace_bytes(const AhFp8Weight* gate_up, const AhFp8Weight* down, int64_t m, size_t* bytes) {
@@ -1133,12 +1330,14 @@ int ah_fp8_ffn(const AhFp8Weight* gate_up, const AhFp8Weight* down, const void* 
   uint8_t* ws = static_cast<uint8_t*>(workspace);
   uint8_t *q1 = ws + l.q1, *q2 = ws + l.q2;
   float *s1 = reinterpret_cast<float*>(ws + l.s1), *s2 = reinterpret_cast<float*>(ws + l.s2);
+  float* partial = l.partial_bytes ? reinterpret_cast<float*>(ws + l.partial) : nullptr;
   rc = ah_fp8_add_rms_norm(x, ldx, residual, ldr, dtype, norm_w, norm_dtype, eps, m, gate_up->cols, q1, l.ldq1, s1,
                            l.lds1, stream);
   if (rc != AH_OK) return rc;
-  rc = matmul_swiglu(gate_up, q1, l.ldq1, s1, l.lds1, m, q2, l.ldq2, s2, l.lds2, as_stream(stream));
+  rc = matmul_swiglu(gate_up, q1, l.ldq1, s1, l.lds1, m, q2, l.ldq2, s2, l.lds2, partial, l.partial_bytes,
+                     as_stream(stream));
   if (rc != AH_OK) return rc;
-  return ah_fp8w_matmul(down, q2, l.ldq2, s2, l.lds2, m, y, ldy, y_dtype, stream);
+  return matmul(down, q2, l.ldq2, s2, l.lds2, m, y, ldy, y_dtype, partial, l.partial_bytes, as_stream(stream));
 }
 
 }  // extern "C"

@@ -173,6 +173,7 @@ class Fp8Weight:
         self._h = handle
         self.rows, self.cols, self.device = rows, cols, device
         self._dev = device.index
+        self._bytes = (-1, 0)  # rows and workspace bytes of the last call
 
     @classmethod
     def _make(cls, name: str, device: torch.device, rows: int, cols: int, *args, n: int | None = None) -> "Fp8Weight":
@@ -201,6 +202,11 @@ class Fp8Weight:
     def weight_bytes(self) -> int:
         return int(lib().ah_fp8w_weight_bytes(self._h))
 
+    def workspace_bytes(self, m: int) -> int:
+        n = C.c_size_t()
+        call("ah_fp8w_matmul_workspace_bytes", self._h, m, C.byref(n))
+        return int(n.value)
+
     def matmul(self, q: torch.Tensor, scales: torch.Tensor, out: torch.Tensor | None = None,
                dtype: torch.dtype = torch.float32) -> torch.Tensor:
         """y = dequant(q, scales) @ W^T, [m, rows] in out's type (or dtype), sums in f32."""
@@ -212,8 +218,13 @@ class Fp8Weight:
         my, ny, ldy = _rows(out, "out", self._dev)
         if my != m or ny != self.rows:
             _refuse(f"out must be [{m}, {self.rows}]")
+        rows, nbytes = self._bytes
+        if rows != m:
+            nbytes = self.workspace_bytes(m)
+            self._bytes = (m, nbytes)
+        ws = torch.empty(nbytes, dtype=torch.uint8, device=self.device) if nbytes else None
         _run(self._dev, "ah_fp8w_matmul", self._h, q.data_ptr(), ldq, scales.data_ptr(), lds, m, out.data_ptr(), ldy,
-             _dtype(out, "out"))
+             _dtype(out, "out"), None if ws is None else ws.data_ptr(), nbytes)
         return out
 
     def close(self):

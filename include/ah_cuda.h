@@ -577,9 +577,15 @@ AH_API int ah_fp8w_shape(const AhFp8Weight* w, int64_t* rows, int64_t* cols);
 AH_API int64_t ah_fp8w_weight_bytes(const AhFp8Weight* w);
 /* y[i][r] = sum over blocks b of 128 columns of scales[i][b] * w_scale[r / 128][b] *
  * (sum over the block of q[i][j] * w[r][j]), sums in f32, rounded once to y_dtype:
- * inference/math.rs:255-295 gemv_4bit_into for m tokens.  y [m][ldy], ldy >= rows. */
+ * inference/math.rs:255-295 gemv_4bit_into for m tokens.  y [m][ldy], ldy >= rows.
+ * The workspace (16-byte aligned, any contents, ah_fp8w_matmul_workspace_bytes, 0
+ * for many shapes) takes the partial sums of tiles split along the columns and
+ * serves one call at a time; with workspace null nothing is split, which is slower
+ * where bytes were asked for and adds in another order. */
+AH_API int ah_fp8w_matmul_workspace_bytes(const AhFp8Weight* w, int64_t m, size_t* bytes);
 AH_API int ah_fp8w_matmul(const AhFp8Weight* w, const uint8_t* q_dev, int64_t ldq, const float* scales_dev,
-                          int64_t lds, int64_t m, void* y_dev, int64_t ldy, uint32_t y_dtype, void* stream);
+                          int64_t lds, int64_t m, void* y_dev, int64_t ldy, uint32_t y_dtype, void* workspace_dev,
+                          size_t workspace_bytes, void* stream);
 /* A feed-forward block (inference/ffn.rs:72-111 with its norm, inference/mod.rs:
  * 505-545): ah_fp8_add_rms_norm of x into residual, gate and up, silu(gate) * up
  * quantised from f32, down: y [m][ldy] = the block's output, which the caller (or

@@ -65,7 +65,8 @@ def test_weight_makers_refuse():
 def test_null_weights_refused():
     L = lib()
     n, i = C.c_size_t(), C.c_int64()
-    assert L.ah_fp8w_matmul(None, P, 208, P, 2, 1, P, 128, 0, None) == EINVAL
+    assert L.ah_fp8w_matmul(None, P, 208, P, 2, 1, P, 128, 0, None, 0, None) == EINVAL
+    assert L.ah_fp8w_matmul_workspace_bytes(None, 1, C.byref(n)) == EINVAL
     assert L.ah_fp8_ffn_workspace_bytes(None, None, 1, C.byref(n)) == EINVAL
     assert L.ah_fp8_ffn(None, None, P, 128, None, 0, 0, P, 1, 1e-5, 1, P, 128, 0, P, 1 << 20, None) == EINVAL
     assert L.ah_fp8w_shape(None, C.byref(i), C.byref(i)) == EINVAL
