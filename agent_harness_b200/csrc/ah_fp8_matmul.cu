@@ -220,6 +220,42 @@ __device__ __forceinline__ void store_y(void* y, int64_t i, uint32_t dtype, floa
   else static_cast<__nv_bfloat16*>(y)[i] = __float2bfloat16_rn(v);
 }
 
+template <typename T>
+__device__ __forceinline__ uint32_t pack2(float a, float b);
+template <>
+__device__ __forceinline__ uint32_t pack2<__half>(float a, float b) {
+  const __half2 h = __floats2half2_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+template <>
+__device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float a, float b) {
+  const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
+  return *reinterpret_cast<const uint32_t*>(&h);
+}
+
+// Values at, at + 1, ... (n of 4) of y: one store where they lie on a boundary of
+// their size.
+__device__ __forceinline__ void store_y4(void* y, int64_t at, uint32_t dtype, const float (&v)[4], int n) {
+  if (dtype == AH_DTYPE_F32) {
+    float* p = static_cast<float*>(y) + at;
+    if (n == 4 && (reinterpret_cast<uintptr_t>(p) & 15) == 0) {
+      *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
+      return;
+    }
+  } else {
+    uint16_t* p = static_cast<uint16_t*>(y) + at;
+    if (n == 4 && (reinterpret_cast<uintptr_t>(p) & 7) == 0) {
+      *reinterpret_cast<uint2*>(p) = dtype == AH_DTYPE_F16
+                                         ? make_uint2(pack2<__half>(v[0], v[1]), pack2<__half>(v[2], v[3]))
+                                         : make_uint2(pack2<__nv_bfloat16>(v[0], v[1]), pack2<__nv_bfloat16>(v[2], v[3]));
+      return;
+    }
+  }
+#pragma unroll
+  for (int i = 0; i < 4; ++i)
+    if (i < n) store_y(y, at + i, dtype, v[i]);
+}
+
 // ---- few tokens: weight rows on the MMA's M, tokens on N ------------------------------
 //
 // A CTA takes one 128-row tile (or a gate/up pair of tiles) and a run of its
@@ -242,6 +278,7 @@ __device__ __forceinline__ void store_y(void* y, int64_t i, uint32_t dtype, floa
 
 constexpr uint32_t kWaitLimit = 1u << 24;
 constexpr int kSmallThreads = 192;
+constexpr int kMaxCluster = 8;
 constexpr int kScaleBlocks = 8;  // column blocks whose scales are staged together
 
 template <int kNt, bool kGlu>
@@ -424,17 +461,18 @@ __global__ void __launch_bounds__(kSmallThreads, 2) k_fp8_small(const __grid_con
     const int q = warp & 3, t = threadIdx.x - 64;  // TMEM lane quarter, reader index
     float* sc = reinterpret_cast<float*>(smem + L::kScale);  // [2][kScaleBlocks][kCols]
     constexpr int kPer = kScaleBlocks * L::kCols / 128;
-    float next[kPer];
-    // thread t's share of the scale products of blocks [i0, i0 + kScaleBlocks):
-    // neighbouring threads take neighbouring blocks of a token
+    float next_a[kPer], next_w[kPer];
+    // thread t's share of the scales of blocks [i0, i0 + kScaleBlocks), multiplied
+    // only when they are put down, eight blocks later; neighbouring threads take
+    // neighbouring blocks of a token
     auto fetch = [&](int i0) {
 #pragma unroll
       for (int j = 0; j < kPer; ++j) {
         const int e = t + j * 128, i = i0 + e % kScaleBlocks, c = e / kScaleBlocks;
         const int64_t tok = m0 + c % kNt;
-        next[j] = i < nb && tok < g.m ? g.ascales[tok * g.lds + b0 + i] *
-                                            g.wscales[(unit * L::kTiles + c / kNt) * g.kb + b0 + i]
-                                      : 0.0f;
+        const bool live = i < nb && tok < g.m;
+        next_a[j] = live ? g.ascales[tok * g.lds + b0 + i] : 0.0f;
+        next_w[j] = live ? g.wscales[(unit * L::kTiles + c / kNt) * g.kb + b0 + i] : 0.0f;
       }
     };
     pdl_wait();  // the scales come from the preceding grid
@@ -450,7 +488,7 @@ __global__ void __launch_bounds__(kSmallThreads, 2) k_fp8_small(const __grid_con
 #pragma unroll
         for (int j = 0; j < kPer; ++j) {
           const int e = t + j * 128;
-          set[e % kScaleBlocks * L::kCols + e / kScaleBlocks] = next[j];
+          set[e % kScaleBlocks * L::kCols + e / kScaleBlocks] = next_a[j] * next_w[j];
         }
         // also: every reader is done with the set before last
         promote_barrier();
@@ -460,24 +498,36 @@ __global__ void __launch_bounds__(kSmallThreads, 2) k_fp8_small(const __grid_con
       tc_fence_after();
       const float* s = set + i % kScaleBlocks * L::kCols;
       const uint32_t ta = tmem + ((uint32_t)(q * 32) << 16) + buf * L::kCols;
-      constexpr int kStep = L::kCols < 32 ? 16 : 32;
+      auto add = [&](int c, float v0, float v1, float v2, float v3) {
+        const float4 f = *reinterpret_cast<const float4*>(s + c);
+        acc[c] = fmaf(v0, f.x, acc[c]);
+        acc[c + 1] = fmaf(v1, f.y, acc[c + 1]);
+        acc[c + 2] = fmaf(v2, f.z, acc[c + 2]);
+        acc[c + 3] = fmaf(v3, f.w, acc[c + 3]);
+      };
+      auto release = [&]() {  // the buffer is read
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(&d_empty[buf]);
+      };
+      if constexpr (L::kCols == 16) {
+        float v[16];
+        tmem_ld16(ta, v);
+        release();
 #pragma unroll
-      for (int c = 0; c < L::kCols; c += kStep) {
-        float v[kStep];
-        if constexpr (kStep == 16) tmem_ld16(ta + c, v);
-        else tmem_ld32(ta + c, v);
+        for (int j = 0; j < 16; j += 4) add(j, v[j], v[j + 1], v[j + 2], v[j + 3]);
+      } else {
+        uint32_t v[L::kCols / 32][32];
 #pragma unroll
-        for (int j = 0; j < kStep; j += 4) {
-          const float4 f = *reinterpret_cast<const float4*>(s + c + j);
-          acc[c + j] = fmaf(v[j], f.x, acc[c + j]);
-          acc[c + j + 1] = fmaf(v[j + 1], f.y, acc[c + j + 1]);
-          acc[c + j + 2] = fmaf(v[j + 2], f.z, acc[c + j + 2]);
-          acc[c + j + 3] = fmaf(v[j + 3], f.w, acc[c + j + 3]);
-        }
+        for (int c = 0; c < L::kCols / 32; ++c) tmem_ld32_issue(ta + c * 32, v[c]);
+#pragma unroll
+        for (int c = 0; c < L::kCols / 32; ++c) tmem_ld32_wait(v[c]);
+        release();
+#pragma unroll
+        for (int c = 0; c < L::kCols; c += 4)
+          add(c, __uint_as_float(v[c / 32][c % 32]), __uint_as_float(v[c / 32][c % 32 + 1]),
+              __uint_as_float(v[c / 32][c % 32 + 2]), __uint_as_float(v[c / 32][c % 32 + 3]));
       }
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(&d_empty[buf]);
       if (++buf == L::kBufs) {
         buf = 0;
         ph ^= 1;
@@ -499,41 +549,44 @@ __global__ void __launch_bounds__(kSmallThreads, 2) k_fp8_small(const __grid_con
   }
   const int live = (int)(g.m - m0 < kNt ? g.m - m0 : kNt);
   if (warp >= 2 && !*abort_flag) {
-    const int t = threadIdx.x - 64;
-    const uint32_t part = smem_u32(smem);
-    if constexpr (kGlu) {
-      // one warp per token: 4 rows per lane, the group's maximum over the warp
-      const int64_t n_ff = g.rows / 2, r = unit * kFp8Group + lane * 4;
-      for (int c = rank + (warp - 2) * nc; c < live; c += 4 * nc) {
-        float gt[4] = {}, up[4] = {};
-        for (int k = 0; k < nc; ++k) {
-          const uint32_t peer = mapa_shared(part, k) + lane * 16;
-          const uint4 a = ld_dsmem_v4(peer + c * 512), b = ld_dsmem_v4(peer + (kNt + c) * 512);
-          gt[0] += __uint_as_float(a.x); gt[1] += __uint_as_float(a.y);
-          gt[2] += __uint_as_float(a.z); gt[3] += __uint_as_float(a.w);
-          up[0] += __uint_as_float(b.x); up[1] += __uint_as_float(b.y);
-          up[2] += __uint_as_float(b.z); up[3] += __uint_as_float(b.w);
-        }
+    // one warp per token, four rows per lane, all members' sums requested at once
+    const uint32_t mine = smem_u32(smem) + lane * 16;
+    auto sum4 = [&](int c, float (&o)[4]) {
+      uint4 v[kMaxCluster];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) gt[i] = r + i < n_ff ? fp8_silu_mul(gt[i], up[i]) : 0.0f;
-        const float fm = max_abs3(max_abs3(kFp8Tiny, gt[0], gt[1]), gt[2], gt[3]);
+      for (int k = 0; k < kMaxCluster; ++k)
+        if (k < nc) v[k] = ld_dsmem_v4(mapa_shared(mine + c * 512, k));
+      o[0] = o[1] = o[2] = o[3] = 0.0f;
+#pragma unroll
+      for (int k = 0; k < kMaxCluster; ++k)
+        if (k < nc) {
+          o[0] += __uint_as_float(v[k].x);
+          o[1] += __uint_as_float(v[k].y);
+          o[2] += __uint_as_float(v[k].z);
+          o[3] += __uint_as_float(v[k].w);
+        }
+    };
+    const int64_t rows = g.gate_up ? g.rows / 2 : g.rows;  // rows of the tile's source
+    const int64_t r = (int64_t)(g.gate_up && !kGlu ? unit >> 1 : unit) * kFp8Group + lane * 4;
+    for (int c = rank + (warp - 2) * nc; c < live; c += 4 * nc) {
+      float o[4];
+      sum4(c, o);
+      if constexpr (kGlu) {
+        float up[4];
+        sum4(kNt + c, up);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) o[i] = r + i < rows ? fp8_silu_mul(o[i], up[i]) : 0.0f;
+        const float fm = max_abs3(max_abs3(kFp8Tiny, o[0], o[1]), o[2], o[3]);
         const float gm = __uint_as_float(__reduce_max_sync(0xFFFFFFFFu, __float_as_uint(fm))), inv = fp8_inverse(gm);
-        const uint32_t w = cvt_e4m3x4(gt[0] * inv, gt[1] * inv, gt[2] * inv, gt[3] * inv);
+        const uint32_t w = cvt_e4m3x4(o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv);
         uint8_t* qrow = p.act_q + (m0 + c) * p.ld_act + r;  // ld_act is a multiple of 16
-        if (r + 4 <= n_ff) *reinterpret_cast<uint32_t*>(qrow) = w;
+        if (r + 4 <= rows) *reinterpret_cast<uint32_t*>(qrow) = w;
         else
-          for (int i = 0; i < 4 && r + i < n_ff; ++i) qrow[i] = (uint8_t)(w >> (8 * i));
+          for (int i = 0; i < 4 && r + i < rows; ++i) qrow[i] = (uint8_t)(w >> (8 * i));
         if (lane == 0) p.act_scales[(m0 + c) * p.lds_act + unit] = gm * (1.0f / kFp8Max);
-      }
-    } else {
-      const int64_t rows = g.gate_up ? g.rows / 2 : g.rows;  // rows of the tile's source
-      const int64_t r0 = (g.gate_up ? unit >> 1 : unit) * kFp8Group, out0 = g.gate_up && (unit & 1) ? rows : 0;
-      // (token, row) elements over the cluster's readers, rows fastest
-      for (int e = rank * 128 + t; e < live * 128; e += nc * 128) {
-        float v = 0.0f;
-        for (int k = 0; k < nc; ++k) v += ld_dsmem_f32(mapa_shared(part, k) + e * 4);
-        const int64_t r = r0 + (e & 127);
-        if (r < rows) store_y(g.y, (m0 + (e >> 7)) * g.ldy + out0 + r, g.y_dtype, v);
+      } else {
+        const int64_t at = (m0 + c) * g.ldy + (g.gate_up && (unit & 1) ? rows : 0) + r;
+        store_y4(g.y, at, g.y_dtype, o, (int)min((int64_t)4, rows - r));
       }
     }
   }
@@ -553,7 +606,7 @@ int device_once(int* dev) {
 // busy, each with two column blocks at least.
 int small_cluster(int64_t units, int64_t kb) {
   int c = 1;
-  while (c < 8 && units * c * 2 <= 2 * sm_count() && kb >= 4 * c) c *= 2;
+  while (c < kMaxCluster && units * c * 2 <= 2 * sm_count() && kb >= 4 * c) c *= 2;
   return c;
 }
 
@@ -596,7 +649,9 @@ int launch_small(SmallArgs& p, cudaStream_t st) {
 
 template <bool kGlu>
 int dispatch_small(SmallArgs& p, cudaStream_t st) {
-  return p.g.m <= 16 ? launch_small<16, kGlu>(p, st) : p.g.m <= 32 ? launch_small<32, kGlu>(p, st) : launch_small<64, kGlu>(p, st);
+  if (p.g.m <= 16) return launch_small<16, kGlu>(p, st);
+  if (kGlu || p.g.m <= 32) return launch_small<32, kGlu>(p, st);
+  if constexpr (!kGlu) return launch_small<64, false>(p, st);
 }
 
 // ---- many tokens: CTA pairs, 256 tokens x 256 weight rows ---------------------------------
@@ -691,19 +746,6 @@ __device__ __forceinline__ void load_scales4(const float* row, int b, int kb, bo
 #pragma unroll
     for (int i = 0; i < 4; ++i) v[i] = b + i < kb ? row[b + i] : 0.0f;
   }
-}
-
-template <typename T>
-__device__ __forceinline__ uint32_t pack2(float a, float b);
-template <>
-__device__ __forceinline__ uint32_t pack2<__half>(float a, float b) {
-  const __half2 h = __floats2half2_rn(a, b);
-  return *reinterpret_cast<const uint32_t*>(&h);
-}
-template <>
-__device__ __forceinline__ uint32_t pack2<__nv_bfloat16>(float a, float b) {
-  const __nv_bfloat162 h = __floats2bfloat162_rn(a, b);
-  return *reinterpret_cast<const uint32_t*>(&h);
 }
 
 template <bool kGlu>
@@ -1139,10 +1181,13 @@ int launch_big(BigArgs& p, const BigPlan& plan, cudaStream_t st) {
   return launch_pdl(k_fp8_join<kGlu>, dim3(chunks, (unsigned)plan.split.rest), dim3(kJoinThreads), 0, st, (const BigArgs)p);
 }
 
-bool use_big(int64_t m) { return m > 64; }
+// Up to 64 tokens (32 for a gate/up pair, whose sums take twice the registers) the
+// weight-streaming kernel is the faster one: 4096 x 4096 at 64 tokens 10.6 us against
+// 13.2, at 32 tokens 8.0 against 13.
+bool use_big(bool glu, int64_t m) { return m > (glu ? 32 : 64); }
 
 // Bytes of partial sums a product of m rows uses.
-size_t matmul_bytes(const AhFp8Weight* w, int64_t m) { return m > 0 && use_big(m) ? big_plan(w, m).bytes : 0; }
+size_t matmul_bytes(const AhFp8Weight* w, bool glu, int64_t m) { return m > 0 && use_big(glu, m) ? big_plan(w, m).bytes : 0; }
 
 int check_matmul(const AhFp8Weight* w, int64_t m) {
   AH_REQUIRE(w, "fp8w_matmul: null weight");
@@ -1155,7 +1200,7 @@ int check_matmul(const AhFp8Weight* w, int64_t m) {
 // The rest of a product's launch, for y or for SwiGLU's outputs (set in p by `set`).
 template <bool kGlu, typename Set>
 int run_matmul(const MatmulArgs& g, const AhFp8Weight* w, float* partial, size_t bytes, cudaStream_t st, Set set) {
-  if (use_big(g.m)) {
+  if (use_big(kGlu, g.m)) {
     BigPlan plan = big_plan(w, g.m);
     AH_REQUIRE(!partial || bytes >= plan.bytes, "fp8w_matmul: workspace of %zu bytes, %zu needed", bytes, plan.bytes);
     if (plan.split.rest && !partial) {  // no workspace: no split
@@ -1230,7 +1275,7 @@ FfnLayout ffn_layout(const AhFp8Weight* gu, const AhFp8Weight* down, int64_t m) 
   l.q2 = l.s1 + up((size_t)m * l.lds1 * 4);
   l.s2 = l.q2 + up((size_t)m * l.ldq2);
   l.partial = l.s2 + up((size_t)m * l.lds2 * 4);
-  l.partial_bytes = std::max(matmul_bytes(gu, m), matmul_bytes(down, m));
+  l.partial_bytes = std::max(matmul_bytes(gu, true, m), matmul_bytes(down, false, m));
   l.total = l.partial + l.partial_bytes;
   return l;
 }
@@ -1297,7 +1342,7 @@ int ah_fp8w_matmul_workspace_bytes(const AhFp8Weight* w, int64_t m, size_t* byte
   const int rc = check_matmul(w, m);
   if (rc != AH_OK) return rc;
   AH_REQUIRE(bytes, "fp8w_matmul_workspace_bytes: null output");
-  *bytes = matmul_bytes(w, m);
+  *bytes = matmul_bytes(w, false, m);
   return AH_OK;
 }
 
