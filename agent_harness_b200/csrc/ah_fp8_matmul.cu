@@ -1181,13 +1181,19 @@ int launch_big(BigArgs& p, const BigPlan& plan, cudaStream_t st) {
   return launch_pdl(k_fp8_join<kGlu>, dim3(chunks, (unsigned)plan.split.rest), dim3(kJoinThreads), 0, st, (const BigArgs)p);
 }
 
-// Up to 64 tokens (32 for a gate/up pair, whose sums take twice the registers) the
-// weight-streaming kernel is the faster one: 4096 x 4096 at 64 tokens 10.6 us against
-// 13.2, at 32 tokens 8.0 against 13.
-bool use_big(bool glu, int64_t m) { return m > (glu ? 32 : 64); }
+// Whether a product goes to the pair kernel.  The weight-streaming kernel takes up
+// to 64 tokens (14336 x 4096 at 64 tokens: 16.4 us against 19.6, a 4096 x 14336
+// feed-forward block 51 against 63), and more while its tiles, one per 64 tokens (32
+// for a gate/up pair), leave clusters of four (two) on two CTAs per SM: 4096 x 4096
+// at 128 tokens 10.6 us against 13.3, but at 192 15.0 against 13.7, and 8192 x 512 at
+// 128 7.2 against 6.1.
+bool use_big(const AhFp8Weight* w, bool glu, int64_t m) {
+  if (m <= 64) return false;
+  return glu ? w->nt / 2 * ((m + 31) / 32) > sm_count() : w->nt * ((m + 63) / 64) > sm_count() / 2;
+}
 
 // Bytes of partial sums a product of m rows uses.
-size_t matmul_bytes(const AhFp8Weight* w, bool glu, int64_t m) { return m > 0 && use_big(glu, m) ? big_plan(w, m).bytes : 0; }
+size_t matmul_bytes(const AhFp8Weight* w, bool glu, int64_t m) { return m > 0 && use_big(w, glu, m) ? big_plan(w, m).bytes : 0; }
 
 int check_matmul(const AhFp8Weight* w, int64_t m) {
   AH_REQUIRE(w, "fp8w_matmul: null weight");
@@ -1200,7 +1206,7 @@ int check_matmul(const AhFp8Weight* w, int64_t m) {
 // The rest of a product's launch, for y or for SwiGLU's outputs (set in p by `set`).
 template <bool kGlu, typename Set>
 int run_matmul(const MatmulArgs& g, const AhFp8Weight* w, float* partial, size_t bytes, cudaStream_t st, Set set) {
-  if (use_big(kGlu, g.m)) {
+  if (use_big(w, kGlu, g.m)) {
     BigPlan plan = big_plan(w, g.m);
     AH_REQUIRE(!partial || bytes >= plan.bytes, "fp8w_matmul: workspace of %zu bytes, %zu needed", bytes, plan.bytes);
     if (plan.split.rest && !partial) {  // no workspace: no split
