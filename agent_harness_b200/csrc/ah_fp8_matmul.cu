@@ -193,6 +193,7 @@ int build(const TileSource (&s)[2], int kind, bool gate_up, int64_t rows, int64_
     destroy(w);
     return fail(AH_ECUDA, "fp8w: building the weight: %s", cudaGetErrorString(e));
   }
+  (void)device_error_word();  // looked up here, so that a product's first call may be captured
   *out = w;
   return AH_OK;
 }
@@ -1050,6 +1051,7 @@ __global__ void __launch_bounds__(kJoinThreads) k_fp8_join(const __grid_constant
   __shared__ float tr[kGlu ? 1 : 32][256 + 1];  // [token][column]
   __shared__ uint32_t maxima[kGlu ? 32 * 32 : 1];
   pdl_launch_dependents();
+  pdl_wait();
   const MatmulArgs& g = p.g;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int mt = (int)((g.m + kBigTokens - 1) / kBigTokens), parts = p.split.parts;
@@ -1063,7 +1065,6 @@ __global__ void __launch_bounds__(kJoinThreads) k_fp8_join(const __grid_constant
   float acc[8];
 #pragma unroll
   for (int j = 0; j < 8; ++j) acc[j] = 0.0f;
-  pdl_wait();
   if (tok < g.m) {
     for (int q = 0; q < parts; q += 4) {  // four pieces' loads in flight
       float v[4][8];
@@ -1169,10 +1170,17 @@ int launch_big(BigArgs& p, const BigPlan& plan, cudaStream_t st) {
   int dev = 0;
   rc = device_once(&dev);
   if (rc != AH_OK) return rc;
+  static int regs[64];
   std::call_once(once[dev], [&] {
     attr[dev] = cudaFuncSetAttribute(k_fp8_big<kGlu>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Big::kDynamic);
+    cudaFuncAttributes a{};
+    if (attr[dev] == cudaSuccess) attr[dev] = cudaFuncGetAttributes(&a, k_fp8_big<kGlu>);
+    regs[dev] = a.numRegs;
   });
   AH_CUDA_TRY(attr[dev]);
+  // raising the readers' registers waits for ever where the launch brought fewer
+  if (regs[dev] * kBigThreads < kBigRegsFew * 128 + kBigRegsMany * 256)
+    return fail(AH_EUNSUPPORTED, "fp8w_matmul: built with %d registers per thread, too few to redistribute", regs[dev]);
   p.split = plan.split;
   rc = launch_pdl(k_fp8_big<kGlu>, dim3((unsigned)(2 * plan.pairs)), dim3(kBigThreads), Big::kDynamic, st,
                   (const BigArgs)p);

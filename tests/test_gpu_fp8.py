@@ -94,12 +94,18 @@ def test_norm(fp8, m, k, dtype, wdtype):
 
 @pytest.mark.parametrize("k", [16384, 20000, 40001])
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
-def test_long_rows(fp8, k, dtype):
-    x, w = randn(3, k, seed=k, dtype=dtype), torch.ones(k, device="cuda")
+@pytest.mark.parametrize("m", [3, 400])
+def test_long_rows(fp8, m, k, dtype):
+    x, w = randn(m, k, seed=k, dtype=dtype), torch.ones(k, device="cuda")
     h = x.double()
     q, s = fp8.add_rms_norm_fp8(x, w)
     check_quantised(q, s, h, 1 / (h.square().mean(1, keepdim=True) + 1e-5).sqrt(), k)
     check_quantised(*fp8.quantize_fp8(x), h)
+    r = randn(m, k, seed=k + 1, dtype=dtype)
+    h = (x.float() + r.float()).to(dtype).double()
+    q, s = fp8.add_rms_norm_fp8(x, w, residual=r)
+    assert torch.equal(r.double(), h)
+    check_quantised(q, s, h, 1 / (h.square().mean(1, keepdim=True) + 1e-5).sqrt(), k)
 
 
 def test_many_short_rows(fp8):
@@ -211,10 +217,94 @@ def test_matmul(fp8, m, n, k):
     W.close()
 
 
-@pytest.mark.parametrize("m", [1, 3, 40, 260])
+# tiles of 256 tokens x 256 rows: one token or row past a tile, odd numbers of weight
+# tiles, one column block and many, outputs a tensor map can and cannot address
+LARGE = [(129, 5000, 130), (300, 4000, 200), (256, 5120, 128), (257, 2433, 1), (513, 2049, 384), (700, 1300, 300),
+         (1025, 1152, 520), (2100, 1003, 257), (4100, 640, 96)]
+
+
+@pytest.mark.parametrize("m,n,k", LARGE)
+def test_matmul_large(fp8, m, n, k):
+    wq, ws = blocks(n, k, m + n + k)
+    W = fp8.Fp8Weight.from_blocks(wq, ws)
+    q, s = acts(fp8, m, k, 1)
+    for dtype in TYPES:
+        check_product(W.matmul(q, s, dtype=dtype), q, s, wq, ws, k)
+    W.close()
+
+
+# tiles past the last full round of the GPU's pairs, cut along the columns
+SPLIT = [(260, 2048, 8192), (300, 1930, 8200), (520, 1200, 6000), (65, 5000, 16000), (2048, 9500, 3200)]
+WHOLE = [(512, 1100, 6000), (65, 4300, 16000)]  # few enough tiles for the other kernel: no workspace
+
+
+@pytest.mark.parametrize("m,n,k", SPLIT + WHOLE)
+def test_matmul_split_along_the_columns(fp8, m, n, k):
+    wq, ws = blocks(n, k, m)
+    W = fp8.Fp8Weight.from_blocks(wq, ws)
+    need = W.workspace_bytes(m)
+    assert (need > 0) == ((m, n, k) in SPLIT)
+    q, s = acts(fp8, m, k, 1)
+    y = W.matmul(q, s)
+    check_product(y, q, s, wq, ws, k)
+    if not need:
+        return
+    check_product(W.matmul(q, s, dtype=torch.bfloat16), q, s, wq, ws, k)
+    assert torch.equal(W.matmul(q, s), y)
+    # no workspace: no split; one too small: refused, nothing written
+    z = torch.full((m, n + 2), -1.0, device="cuda")
+    st = torch.cuda.current_stream().cuda_stream
+    ws_ = torch.full((need,), 0xFF, dtype=torch.uint8, device="cuda")
+
+    def call(workspace, nbytes):
+        return lib().ah_fp8w_matmul(W.handle, q.data_ptr(), q.stride(0), s.data_ptr(), s.stride(0), m, z.data_ptr(),
+                                    n + 2, 0, workspace, nbytes, st)
+
+    assert call(ws_.data_ptr(), need - 1) == -1 and call(ws_.data_ptr() + 4, need) == -1
+    assert (z == -1).all()
+    assert call(None, 0) == 0
+    check_product(z[:, :n], q, s, wq, ws, k)
+    z.fill_(-1)
+    assert call(ws_.data_ptr(), need) == 0  # NaN bit patterns in the workspace
+    assert torch.equal(z[:, :n], y) and (z[:, n:] == -1).all()
+    W.close()
+
+
+@pytest.mark.parametrize("m,n_embd,n_ff", [(300, 8192, 1000), (400, 700, 2500), (1500, 256, 1100), (320, 8000, 2000)])
+def test_gate_up_weight_as_a_plain_one(fp8, m, n_embd, n_ff):
+    """gate | up in one product, whole and split tiles, n_ff not a multiple of 128."""
+    (gq, gs), (uq, us), (dq, ds) = ffn_weights(n_embd, n_ff, m)
+    block = fp8.Fp8SwigluBlock.from_blocks(gq, gs, uq, us, dq, ds)
+    q, s = acts(fp8, m, n_embd, 3)
+    for dtype in TYPES:
+        gu = block.gate_up.matmul(q, s, dtype=dtype)
+        check_product(gu[:, :n_ff], q, s, gq, gs, n_embd)
+        check_product(gu[:, n_ff:], q, s, uq, us, n_embd)
+    block.close()
+
+
+@pytest.mark.parametrize("m,n", [(5, 300), (300, 2100), (700, 1500)])
+def test_infinite_scales_and_huge_values(fp8, m, n):
+    """Scales and sums near the ends of f32 behave as f32 does: an infinite activation
+    scale makes its row infinite or NaN, every other row stays finite."""
+    k = 512
+    wq, ws = blocks(n, k, 2)
+    W = fp8.Fp8Weight.from_blocks(wq, ws)
+    q, s = acts(fp8, m, k, 3)
+    s = s.clone()
+    s[2, 1] = float("inf")
+    y = W.matmul(q, s)
+    rest = torch.ones(m, dtype=torch.bool, device="cuda")
+    rest[2] = False
+    assert not torch.isfinite(y[2]).any() and torch.isfinite(y[rest]).all()
+    s[2, 1] = 1.0
+    check_product(W.matmul(q, s), q, s, wq, ws, k)
+
+
+@pytest.mark.parametrize("m", [1, 3, 40, 260, 900])
 def test_matmul_strides_and_rows_behind(fp8, m):
     """Unaligned weight rows, padded activations and scales, an output inside a larger matrix."""
-    n, k = 300, 500
+    n, k = (300, 500) if m < 900 else (1500, 500)
     wq, ws = blocks(n, k + 3, 5)
     wq, ws = wq[:, 1:k + 1], ws
     W = fp8.Fp8Weight.from_blocks(wq, ws)
@@ -252,10 +342,10 @@ def test_weight_from_float(fp8, n, k, dtype):
     W.close()
 
 
-@pytest.mark.parametrize("m", [1, 5, 70, 300])
+@pytest.mark.parametrize("m", [1, 5, 70, 300, 1300])
 def test_non_finite_rows_stay_theirs(fp8, m):
     """A NaN in one token's values or scales, or in one weight row, reaches only its outputs."""
-    n, k = 400, 384
+    n, k = (400, 384) if m < 300 else (2100, 384)
     wq, ws = blocks(n, k, 8)
     wb = wq.view(torch.uint8).clone()
     wb[270, 200] = 0x7F
@@ -308,7 +398,7 @@ def ffn_weights(n_embd, n_ff, seed):
 
 
 FFN = [(1, 256, 384), (1, 1024, 2048), (3, 130, 200), (16, 512, 700), (40, 200, 1000), (130, 384, 512),
-       (300, 640, 1030), (600, 256, 300)]
+       (300, 640, 1030), (600, 256, 300), (320, 8192, 2000), (520, 300, 2200)]
 
 
 @pytest.mark.parametrize("m,n_embd,n_ff", FFN)
@@ -429,10 +519,57 @@ def test_capture_and_streams(fp8, m):
 
 
 def test_repeats_are_bit_identical(fp8):
-    for m, n, k in [(1, 4096, 4096), (16, 1000, 2048), (100, 700, 900), (400, 1100, 1500)]:
+    for m, n, k in [(1, 4096, 4096), (16, 1000, 2048), (100, 700, 900), (400, 2500, 1500), (260, 2048, 8192)]:
         wq, ws = blocks(n, k, 3)
         W = fp8.Fp8Weight.from_blocks(wq, ws)
         q, s = acts(fp8, m, k, 4)
         y = W.matmul(q, s)
         for _ in range(5):
             assert torch.equal(W.matmul(q, s), y)
+
+
+_FRESH = """
+import sys, torch
+sys.path.insert(0, sys.argv[1])
+from agent_harness_b200 import fp8
+d, n, m = 512, 1024, int(sys.argv[2])
+g = torch.Generator("cuda").manual_seed(1)
+block = fp8.Fp8SwigluBlock.from_float(*[torch.randn(*s, generator=g, device="cuda") for s in ((n, d), (n, d), (d, n))])
+x, r, w = torch.randn(m, d, generator=g, device="cuda"), torch.zeros(m, d, device="cuda"), torch.ones(d, device="cuda")
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    y = block(x, w, residual=r)
+graph.replay()
+want = block(x, w, residual=torch.zeros_like(r))
+torch.cuda.synchronize()
+assert torch.equal(y, want), "captured and eager differ"
+"""
+
+
+@pytest.mark.parametrize("m", [1, 2000])
+def test_first_call_may_be_captured(fp8, m):
+    """A fresh process whose first products are captured, without an eager call before."""
+    import os
+    import subprocess
+    import sys
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, "-c", _FRESH, root, str(m)], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0, r.stdout + r.stderr
+
+
+def test_operators_on_unlike_streams(fp8):
+    """Inputs made on one stream, used on another that waits for it, outputs read on a third."""
+    a, b = torch.cuda.Stream(), torch.cuda.Stream()
+    wq, ws = blocks(700, 512, 4)
+    W = fp8.Fp8Weight.from_blocks(wq, ws)
+    with torch.cuda.stream(a):
+        x = randn(50, 512, seed=6)
+        q, s = fp8.quantize_fp8(x)
+    b.wait_stream(a)
+    with torch.cuda.stream(b):
+        y = W.matmul(q, s)
+    torch.cuda.current_stream().wait_stream(b)
+    for t in (x, q, s, y):
+        t.record_stream(torch.cuda.current_stream())
+    check_quantised(q, s, x.double())
+    check_product(y, q, s, wq, ws, 512)
