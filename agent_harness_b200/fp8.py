@@ -18,7 +18,7 @@ from ._lib import AhError, call, check, lib
 
 GROUP = 128
 _DTYPES = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 30}
-_E4M3 = torch.float8_e4m3fn
+_E4M3, _F32 = torch.float8_e4m3fn, torch.float32
 
 
 def _refuse(message: str):
@@ -28,23 +28,33 @@ def _refuse(message: str):
 # The checks below run on every call of a decode step, beside kernels of a few
 # microseconds: they read each tensor attribute once, and compare devices by index.
 
-def _rows(t: torch.Tensor, what: str, device: int | None = None) -> tuple[int, int, int]:
-    """(rows, columns, row stride) of a CUDA matrix with unit-stride columns."""
-    shape = t.shape
-    dev = t.get_device()
+def _rows(t: torch.Tensor, what: str) -> tuple[int, int, int, int]:
+    """(rows, columns, row stride, device) of a CUDA matrix with unit-stride columns."""
+    shape, dev = t.shape, t.get_device()
     if len(shape) != 2 or dev < 0:
         _refuse(f"{what}: expected a CUDA matrix")
-    if device is not None and dev != device:
-        _refuse(f"{what}: on another device than the other tensors")
     m, k = shape
+    return m, k, k if t.is_contiguous() else _stride(t, m, k, what), dev
+
+
+def _stride(t: torch.Tensor, m: int, k: int, what: str) -> int:
     ld, unit = t.stride()
     if unit != 1 and k > 1:
         _refuse(f"{what}: expected unit-stride columns")
     if ld < k:
         if m > 1:
             _refuse(f"{what}: rows overlap")
-        ld = k  # a single row's stride is free
-    return m, k, ld
+        return k  # a single row's stride is free
+    return ld
+
+
+def _like(t: torch.Tensor, m: int, k: int, device: int, what: str) -> int:
+    """The row stride of a second matrix, which has to be [m, k] on that device."""
+    if t.shape != (m, k):
+        _refuse(f"{what}: expected [{m}, {k}], got {list(t.shape)}")
+    if t.get_device() != device:
+        _refuse(f"{what}: on another device than the other tensors")
+    return k if t.is_contiguous() else _stride(t, m, k, what)
 
 
 def _dtype(t: torch.Tensor, what: str) -> int:
@@ -54,17 +64,12 @@ def _dtype(t: torch.Tensor, what: str) -> int:
     return code
 
 
-def _quantised(q: torch.Tensor, scales: torch.Tensor, device: int) -> tuple[int, int, int, int]:
-    """Checks a (q, scales) pair: (rows, columns, their row strides)."""
-    m, k, ldq = _rows(q, "q", device)
-    ms, ks, lds = _rows(scales, "scales", device)
-    if q.dtype is not _E4M3 or scales.dtype is not torch.float32:
+def _quantised(q: torch.Tensor, scales: torch.Tensor, m: int, k: int, device: int) -> tuple[int, int]:
+    """Checks a (q, scales) pair of m rows and k columns: their row strides."""
+    if q.dtype is not _E4M3 or scales.dtype is not _F32:
         _refuse("expected q as float8_e4m3fn and scales as float32")
-    if ms != m or ks != (k + 127) // 128:
-        _refuse("scales must be [rows, ceil(columns / 128)]")
-    if m <= 1:
-        ldq = (ldq + 15) // 16 * 16
-    return m, k, ldq, lds
+    ldq, lds = _like(q, m, k, device, "q"), _like(scales, m, (k + 127) // 128, device, "scales")
+    return (ldq + 15) // 16 * 16 if m == 1 else ldq, lds
 
 
 def alloc(m: int, k: int, device="cuda") -> tuple[torch.Tensor, torch.Tensor]:
@@ -74,16 +79,11 @@ def alloc(m: int, k: int, device="cuda") -> tuple[torch.Tensor, torch.Tensor]:
 
 
 def _outputs(m: int, k: int, device: int, out, scales):
-    if out is None:
-        if scales is not None:
+    if out is None or scales is None:
+        if out is not scales:
             _refuse("give out and scales together")
         out, scales = alloc(m, k, torch.device("cuda", device))
-        return out, scales, (k + 15) // 16 * 16, (k + 127) // 128
-    if scales is None:
-        _refuse("give out and scales together")
-    mo, ko, ldq, lds = _quantised(out, scales, device)
-    if mo != m or ko != k:
-        _refuse("out must have the input's shape")
+    ldq, lds = _quantised(out, scales, m, k, device)
     return out, scales, ldq, lds
 
 
@@ -108,8 +108,8 @@ def _run(device: int, name: str, *args):
 def quantize_fp8(x: torch.Tensor, out: torch.Tensor | None = None,
                  scales: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
     """x [m, k] f32 / f16 / bf16 -> (q, scales)."""
-    m, k, ldx = _rows(x, "x")
-    dt, dev = _dtype(x, "x"), x.get_device()
+    m, k, ldx, dev = _rows(x, "x")
+    dt = _dtype(x, "x")
     out, scales, ldq, lds = _outputs(m, k, dev, out, scales)
     _run(dev, "ah_fp8_quantize", x.data_ptr(), ldx, dt, m, k, out.data_ptr(), ldq, scales.data_ptr(), lds)
     return out, scales
@@ -119,11 +119,10 @@ def swiglu_fp8(gate: torch.Tensor, up: torch.Tensor, out: torch.Tensor | None = 
                scales: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
     """silu(gate) * up (inference/ffn.rs:155-174), quantised: gate and up [m, k] of
     one type (halves of one matrix will do) -> (q, scales)."""
-    m, k, ldg = _rows(gate, "gate")
-    dt, dev = _dtype(gate, "gate"), gate.get_device()
-    mu, ku, ldu = _rows(up, "up", dev)
-    if mu != m or ku != k or up.dtype is not gate.dtype:
-        _refuse("gate and up must have one shape and type")
+    m, k, ldg, dev = _rows(gate, "gate")
+    dt, ldu = _dtype(gate, "gate"), _like(up, m, k, dev, "up")
+    if up.dtype is not gate.dtype:
+        _refuse("gate and up must have one type")
     out, scales, ldq, lds = _outputs(m, k, dev, out, scales)
     _run(dev, "ah_fp8_swiglu", gate.data_ptr(), ldg, up.data_ptr(), ldu, dt, m, k, out.data_ptr(), ldq,
          scales.data_ptr(), lds)
@@ -131,17 +130,15 @@ def swiglu_fp8(gate: torch.Tensor, up: torch.Tensor, out: torch.Tensor | None = 
 
 
 def _norm_args(x, norm_w, residual):
-    m, k, ldx = _rows(x, "x")
-    dt, dev, wdt = _dtype(x, "x"), x.get_device(), _dtype(norm_w, "norm_w")
-    if norm_w.shape != (k,) or not norm_w.is_contiguous() or norm_w.get_device() != dev:
+    m, k, ldx, dev = _rows(x, "x")
+    dt, wdt = _dtype(x, "x"), _dtype(norm_w, "norm_w")
+    if norm_w.shape != (k,) or norm_w.get_device() != dev or not norm_w.is_contiguous():
         _refuse("norm_w must be one contiguous value per column, on x's device")
-    rp, ldr = None, 0
-    if residual is not None:
-        mr, kr, ldr = _rows(residual, "residual", dev)
-        if mr != m or kr != k or residual.dtype is not x.dtype:
-            _refuse("residual must have x's shape and type")
-        rp = residual.data_ptr()
-    return m, k, dev, ldx, dt, wdt, rp, ldr
+    if residual is None:
+        return m, k, dev, ldx, dt, wdt, None, 0
+    if residual.dtype is not x.dtype:
+        _refuse("residual must have x's type")
+    return m, k, dev, ldx, dt, wdt, residual.data_ptr(), _like(residual, m, k, dev, "residual")
 
 
 def add_rms_norm_fp8(x: torch.Tensor, norm_w: torch.Tensor, residual: torch.Tensor | None = None, eps: float = 1e-5,
@@ -158,12 +155,10 @@ def add_rms_norm_fp8(x: torch.Tensor, norm_w: torch.Tensor, residual: torch.Tens
 
 
 def _blocks_of(q: torch.Tensor, scales: torch.Tensor) -> tuple[int, int]:
-    ldq, lds = _rows(q, "q")[2], _rows(scales, "scales", q.get_device())[2]
-    if q.dtype != _E4M3 or scales.dtype != torch.float32:
+    n, k, ldq, dev = _rows(q, "q")
+    if q.dtype is not _E4M3 or scales.dtype is not _F32:
         _refuse("expected q as float8_e4m3fn and scales as float32")
-    if scales.shape != tuple((n + GROUP - 1) // GROUP for n in q.shape):
-        _refuse("scales must be [ceil(rows / 128), ceil(columns / 128)]")
-    return ldq, lds
+    return ldq, _like(scales, (n + GROUP - 1) // GROUP, (k + GROUP - 1) // GROUP, dev, "scales")
 
 
 class Fp8Weight:
@@ -210,20 +205,18 @@ class Fp8Weight:
     def matmul(self, q: torch.Tensor, scales: torch.Tensor, out: torch.Tensor | None = None,
                dtype: torch.dtype = torch.float32) -> torch.Tensor:
         """y = dequant(q, scales) @ W^T, [m, rows] in out's type (or dtype), sums in f32."""
-        m, k, ldq, lds = _quantised(q, scales, self._dev)
-        if k != self.cols:
-            _refuse(f"q must be [m, {self.cols}]")
+        shape, dev = q.shape, self._dev
+        m = shape[0] if len(shape) == 2 else -1
+        ldq, lds = _quantised(q, scales, m, self.cols, dev)
         if out is None:
             out = torch.empty(m, self.rows, dtype=dtype, device=self.device)
-        my, ny, ldy = _rows(out, "out", self._dev)
-        if my != m or ny != self.rows:
-            _refuse(f"out must be [{m}, {self.rows}]")
+        ldy = _like(out, m, self.rows, dev, "out")
         rows, nbytes = self._bytes
         if rows != m:
             nbytes = self.workspace_bytes(m)
             self._bytes = (m, nbytes)
         ws = torch.empty(nbytes, dtype=torch.uint8, device=self.device) if nbytes else None
-        _run(self._dev, "ah_fp8w_matmul", self._h, q.data_ptr(), ldq, scales.data_ptr(), lds, m, out.data_ptr(), ldy,
+        _run(dev, "ah_fp8w_matmul", self._h, q.data_ptr(), ldq, scales.data_ptr(), lds, m, out.data_ptr(), ldy,
              _dtype(out, "out"), None if ws is None else ws.data_ptr(), nbytes)
         return out
 
@@ -294,9 +287,7 @@ class Fp8SwigluBlock:
             _refuse(f"x must be [m, {self.n_embd}] on {self.device}")
         if out is None:
             out = torch.empty(m, k, dtype=x.dtype, device=self.device)
-        my, ny, ldy = _rows(out, "out", dev)
-        if my != m or ny != k:
-            _refuse("out must have x's shape")
+        ldy = _like(out, m, k, dev, "out")
         rows, nbytes = self._bytes
         if rows != m:
             nbytes = self.workspace_bytes(m)
