@@ -262,9 +262,9 @@ __device__ __forceinline__ void store_y4(void* y, int64_t at, uint32_t dtype, co
 // A CTA takes one 128-row tile (or a gate/up pair of tiles) and a run of its
 // column blocks for kNt tokens; a cluster of up to 8 CTAs shares a tile's column
 // blocks and adds its members' sums through distributed shared memory in rank
-// order.
+// order, so results do not depend on timing.
 //
-//   warp 0     producer: one bulk copy of KS column blocks of weights per stage
+//   warp 0     producer: one bulk copy of kKs column blocks of weights per stage
 //              (contiguous, 16 or 32 KB each) and a TMA box of each block's tokens
 //   warp 1     TMEM owner, MMA issuer: M = 128, N = kNt, K = 32, four per block
 //   warps 2-5  a block's sums from tensor memory, times a_scale * w_scale, added
@@ -273,9 +273,13 @@ __device__ __forceinline__ void store_y4(void* y, int64_t at, uint32_t dtype, co
 // A block's sums are overwritten, not accumulated, in tensor memory: the scales
 // change with every block.  kBufs buffers let the MMAs run ahead of the readers.
 //
-// Bound by the weight stream: the first stages' weights are requested before the
-// kernel waits for the grid ahead of it (a weight is complete once its handle
-// exists).
+// Bound by the weight stream (a token costs it nothing up to 32): the first stages'
+// weights are requested before the kernel waits for the grid ahead of it (a weight
+// is complete once its handle exists), and two CTAs per SM keep 200 KB in flight.
+// 128256 x 4096 at 16 tokens 87 us (6.1 TB/s), 28672 x 8192 at one 39 us (6.0), 4096 x
+// 4096 at one 5.7 us (3.0: launch, first copies and the cluster's sum take 3 us).  At
+// 64 tokens the shared memory's bandwidth is the bound (operands twice, and a
+// broadcast read of four scales per four columns): 14336 x 4096 16.3 us (3.8 TB/s).
 
 constexpr uint32_t kWaitLimit = 1u << 24;
 constexpr int kSmallThreads = 192;
@@ -669,6 +673,17 @@ int dispatch_small(SmallArgs& p, cudaStream_t st) {
 //              weight tile: sums times a_scale * w_scale into 128 f32 registers,
 //              one multiply-add each, since w_scale is one number per weight tile
 //              and column block; then the tile's output
+//
+// What bounds it: a column block's MMAs take 560 cycles, and a buffer's way round
+// (MMAs, the commit's way to both CTAs, the readers, their arrivals' way back) 1700 to
+// 1800, hidden by two buffers down to 850 to 900.  Readers that hand the buffers back
+// unread leave 570 cycles and 333 us for 2048 x 28672 x 8192, where the kernel takes 414
+// (2322 TFLOP/s; sustained, the power cap leaves 2000).  Measured and not kept: half
+// buffers of N = 128 (452 us) and tiles of one weight tile with four buffers (506),
+// both bound by the readers' fixed cost per wait; single CTAs of 128 x 256 (443, half as
+// much again to load); scales through shared memory (427).  A release of cluster scope
+// on the arrivals cost a memory barrier each (939 against 598 us at the time), issuing
+// copies and MMAs outside uniform code another third.
 
 constexpr int kBigStages = 6;
 constexpr int kBigThreads = 384;

@@ -12,6 +12,13 @@
 // its data, without waiting for the row's sum.  All arithmetic is f32; each z
 // is rounded once, to e4m3.
 //
+// Bound by HBM once there are rows enough: 16384 x 8192 bf16 with a residual 144 us
+// (6.5 TB/s, a copy's rate), 2048 x 28672 bf16 SwiGLU 47 us (6.3 TB/s).  A group is 16 or
+// 32 neighbouring lanes' 16-byte pieces, so its maximum is a few shuffles and nothing
+// waits for another warp but a norm row's sum.  One row of 4096 takes 2.3 us, a launch's
+// latency.  Rows that do not start at multiples of 16 bytes are read by elements, at a
+// third to two thirds of the rate.
+//
 // A group's maximum keeps a NaN, and an infinite one has a NaN inverse: a group
 // with a NaN or an infinity comes out as NaN.
 #include <algorithm>
