@@ -88,19 +88,18 @@ def _outputs(m: int, k: int, device: int, out, scales):
 
 
 _functions: dict = {}
+_current_device = torch._C._cuda_getDevice  # what torch.cuda.current_device and current_stream return,
+_raw_stream = torch._C._cuda_getCurrentRawStream  # without their wrappers
 
 
 def _run(device: int, name: str, *args):
     """One library call on the device's current stream."""
-    fn = _functions.get(name)
-    if fn is None:
-        fn = _functions[name] = getattr(lib(), name)
-    stream = torch._C._cuda_getCurrentRawStream(device)
-    if torch._C._cuda_getDevice() == device:
-        rc = fn(*args, stream)
+    fn = _functions.get(name) or _functions.setdefault(name, getattr(lib(), name))
+    if _current_device() == device:
+        rc = fn(*args, _raw_stream(device))
     else:
         with torch.cuda.device(device):
-            rc = fn(*args, stream)
+            rc = fn(*args, _raw_stream(device))
     if rc:
         check(rc)
 
