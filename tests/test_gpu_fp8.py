@@ -108,6 +108,29 @@ def test_long_rows(fp8, m, k, dtype):
     check_quantised(q, s, h, 1 / (h.square().mean(1, keepdim=True) + 1e-5).sqrt(), k)
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("m,k", [(3, 5), (4, 24), (2, 263), (9, 1030), (301, 517)])
+def test_norm_rows_at_every_alignment(fp8, m, k, dtype):
+    """Rows of x, residual and w that start at any element of a 16-byte piece, row strides
+    odd and even; what lies around the residual's rows stays as it was."""
+    for i in range(9):
+        for j in (0, 1, 3, 6):
+            stride = k + 11 + (i + j) % 3
+            xs, rs = randn(m, stride, seed=i, dtype=dtype), randn(m, stride + 1, seed=j + 50, dtype=dtype)
+            x, r = xs[:, i:i + k], rs[:, j:j + k]
+            w = (1 + 0.2 * randn(k + i, seed=3)).to(dtype)[i // 2:i // 2 + k]
+            h = (x.float() + r.float()).to(dtype).double()
+            around = rs.clone()
+            around[:, j:j + k] = h.to(dtype)
+            q, s = fp8.add_rms_norm_fp8(x, w, residual=r)
+            assert torch.equal(rs, around)
+            rms = 1 / (h.square().mean(1, keepdim=True) + 1e-5).sqrt()
+            check_quantised(q, s, h * w.double(), rms, k)
+            q, s = fp8.add_rms_norm_fp8(x, w)
+            rms = 1 / (x.double().square().mean(1, keepdim=True) + 1e-5).sqrt()
+            check_quantised(q, s, x.double() * w.double(), rms, k)
+
+
 def test_many_short_rows(fp8):
     """More rows than a grid's second dimension holds."""
     m, k = 70001, 24
