@@ -216,7 +216,7 @@ struct RowArgs {
 
 constexpr int kRowThreads = 256;
 
-// One row and 256 * kN * kV columns per CTA, or kNarrow: blockDim.y rows of one piece
+// One row and 256 * kN * kV columns per CTA, or kNarrow: kN * blockDim.y rows of one piece
 // per thread (blockDim.x is a multiple of 32).  A thread requests its kN pieces of
 // every input before it uses the first.
 template <int kMode, typename T, bool kVec, bool kNarrow, int kN>
@@ -224,21 +224,22 @@ __global__ void __launch_bounds__(kRowThreads) k_fp8_rows(const RowArgs g) {
   constexpr int kV = Vec<T>::kV;
   pdl_launch_dependents();
   pdl_wait();
-  const int ty = kNarrow ? (int)blockDim.y : 1;
+  const int ty = kNarrow ? (int)blockDim.y : 1, rows = kNarrow ? kN * ty : 1;
   const int c0 = (kNarrow ? (int)threadIdx.x : (int)(blockIdx.x * kN * kRowThreads + threadIdx.x)) * kV;
-  for (int64_t row = (int64_t)blockIdx.y * ty + (kNarrow ? threadIdx.y : 0); row < g.m; row += (int64_t)gridDim.y * ty) {
-    const T* arow = static_cast<const T*>(g.a) + row * g.lda;
-    const T* brow = static_cast<const T*>(g.b) + row * g.ldb;
+  for (int64_t r0 = (int64_t)blockIdx.y * rows + (kNarrow ? threadIdx.y : 0); r0 < g.m; r0 += (int64_t)gridDim.y * rows) {
     uint4 pa[kN], pb[kMode == kRowSwiglu ? kN : 1];
 #pragma unroll
     for (int i = 0; i < kN; ++i) {
-      const int c = c0 + i * kRowThreads * kV;
-      pa[i] = load_piece<kVec, false>(arow, c, g.k);
-      if constexpr (kMode == kRowSwiglu) pb[i] = load_piece<kVec, false>(brow, c, g.k);
+      const int64_t row = kNarrow ? min(r0 + i * ty, g.m - 1) : r0;  // past the last row: read, not stored
+      const int c = kNarrow ? c0 : c0 + i * kRowThreads * kV;
+      pa[i] = load_piece<kVec, false>(static_cast<const T*>(g.a) + row * g.lda, c, g.k);
+      if constexpr (kMode == kRowSwiglu)
+        pb[i] = load_piece<kVec, false>(static_cast<const T*>(g.b) + row * g.ldb, c, g.k);
     }
 #pragma unroll
     for (int i = 0; i < kN; ++i) {
-      const int c = c0 + i * kRowThreads * kV;
+      const int64_t row = kNarrow ? r0 + i * ty : r0;
+      const int c = kNarrow ? c0 : c0 + i * kRowThreads * kV;
       float z[kV];
       unpack<T>(pa[i], z);
       if constexpr (kMode == kRowSwiglu) {
@@ -248,7 +249,7 @@ __global__ void __launch_bounds__(kRowThreads) k_fp8_rows(const RowArgs g) {
         for (int j = 0; j < kV; ++j) z[j] = fp8_silu_mul(z[j], u[j]);
       }
       const float gm = group_max<T>(z);
-      if (c < g.k) {
+      if (c < g.k && row < g.m) {
         store_q<kVec>(g.q + row * g.ldq, c, g.k, z, fp8_inverse(gm));
         if (c % kFp8Group == 0) g.scales[row * g.lds + c / kFp8Group] = gm * (1.0f / kFp8Max);
       }
@@ -411,16 +412,23 @@ bool vec_rows(const void* p, int64_t ld, uint32_t dtype) {
 
 template <int kMode, typename T>
 int launch_rows(const RowArgs& g, bool vec, cudaStream_t st) {
-  // Narrow rows share a CTA; wide ones take two pieces per thread once that still
-  // leaves every SM four CTAs (16384 x 8192 bf16 SwiGLU: 104 us with two, 120 with one).
   const int64_t pieces = (g.k + Vec<T>::kV - 1) / Vec<T>::kV;
   vec = vec && g.k % Vec<T>::kV == 0;
-  if (pieces <= kRowThreads / 2) {
+  if (pieces <= kRowThreads) {
+    // Narrow rows share a CTA, and a thread takes a piece of kRows rows once that leaves every
+    // SM four CTAs.  16384 x 2048 bf16 quantise: 18.1 us with four, 19.9 with two, 24.7 with
+    // one; 16384 x 1024 f32 SwiGLU 25.4, 24.6, 27.1; 16384 x 2048 bf16 SwiGLU 35.1, 32.7, 29.0.
+    constexpr int kRows = kMode == kRowQuantize ? 4 : sizeof(T) == 4 ? 2 : 1;
     const unsigned tx = (unsigned)((pieces + 31) / 32 * 32), ty = kRowThreads / tx;
-    const dim3 grid(1, (unsigned)std::min<int64_t>((g.m + ty - 1) / ty, 65535));
-    return launch_pdl(vec ? k_fp8_rows<kMode, T, true, true, 1> : k_fp8_rows<kMode, T, false, true, 1>, grid,
-                      dim3(tx, ty), 0, st, g);
+    const bool many = vec && g.m >= (int64_t)kRows * ty * 4 * sm_count();
+    const int64_t rows = (many ? kRows : 1) * ty;
+    const dim3 grid(1, (unsigned)std::min<int64_t>((g.m + rows - 1) / rows, 65535));
+    return launch_pdl(many ? k_fp8_rows<kMode, T, true, true, kRows>
+                      : vec ? k_fp8_rows<kMode, T, true, true, 1> : k_fp8_rows<kMode, T, false, true, 1>,
+                      grid, dim3(tx, ty), 0, st, g);
   }
+  // Wide ones take two pieces per thread once that still leaves every SM four CTAs
+  // (16384 x 8192 bf16 SwiGLU: 104 us with two, 120 with one).
   const bool many = vec && g.m * ((pieces + 2 * kRowThreads - 1) / (2 * kRowThreads)) >= 4 * (int64_t)sm_count();
   const int64_t cols = (int64_t)kRowThreads * (many ? 2 : 1);
   const dim3 grid((unsigned)((pieces + cols - 1) / cols), (unsigned)std::min<int64_t>(g.m, 65535));

@@ -131,6 +131,24 @@ def test_norm_rows_at_every_alignment(fp8, m, k, dtype):
             check_quantised(q, s, x.double() * w.double(), rms, k)
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("m,k", [(2401, 1024), (2403, 1032), (19001, 128), (9502, 264), (4999, 2048)])
+def test_many_narrow_rows(fp8, m, k, dtype):
+    """Several rows per thread, row counts that leave some of them empty."""
+    n = m + 3
+    q = torch.full((n, (k + 15) // 16 * 16), 7, dtype=torch.uint8, device="cuda").view(torch.float8_e4m3fn)
+    s = torch.full((n, (k + G - 1) // G), -1.0, device="cuda")
+    x, u = randn(m, k, seed=m, dtype=dtype), randn(m, k, seed=k, dtype=dtype)
+    g = x.double()
+    for z in (g, g / (1 + torch.exp(-g)) * u.double()):
+        if z is g:
+            fp8.quantize_fp8(x, out=q[:m, :k], scales=s[:m])
+        else:
+            fp8.swiglu_fp8(x, u, out=q[:m, :k], scales=s[:m])
+        check_quantised(q[:m, :k], s[:m], z)
+        assert (q.view(torch.uint8)[m:] == 7).all() and (s[m:] == -1).all()
+
+
 def test_many_short_rows(fp8):
     """More rows than a grid's second dimension holds."""
     m, k = 70001, 24
