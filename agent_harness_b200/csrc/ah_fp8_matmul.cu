@@ -674,36 +674,44 @@ int dispatch_small(SmallArgs& p, cudaStream_t st) {
 //              one multiply-add each, since w_scale is one number per weight tile
 //              and column block; then the tile's output
 //
+// Up to 128 tokens (!kPair) single CTAs walk tiles of 128 tokens x two weight tiles,
+// loading both images (48 KB per column block, M = 128): half of a pair's rows would be
+// empty.  128 x 28672 x 8192 45 us (5.2 TB/s of weights; pairs 66), 128 x 32000 x 2048
+// 16.7 (24), a 4096 x 14336 feed-forward block at 128 tokens 53 (65).  Past 128 tokens
+// single CTAs load half as much again: 443 us where pairs take 414.
+//
 // What bounds it: a column block's MMAs take 560 cycles, and a buffer's way round
 // (MMAs, the commit's way to both CTAs, the readers, their arrivals' way back) 1700 to
-// 1800, hidden by two buffers down to 850 to 900.  Readers that hand the buffers back
-// unread leave 570 cycles and 333 us for 2048 x 28672 x 8192, where the kernel takes 414
-// (2322 TFLOP/s; sustained, the power cap leaves 2000).  Measured and not kept: half
-// buffers of N = 128 (452 us) and tiles of one weight tile with four buffers (506),
-// both bound by the readers' fixed cost per wait; single CTAs of 128 x 256 (443, half as
-// much again to load); scales through shared memory (427).  A release of cluster scope
-// on the arrivals cost a memory barrier each (939 against 598 us at the time), issuing
-// copies and MMAs outside uniform code another third.
+// 1800, hidden by two buffers down to 850 to 900.  2048 x 28672 x 8192 takes 414 us (2322
+// TFLOP/s; sustained, the power cap leaves 2000).  Readers that only read tensor memory
+// leave 373 us, that only multiply and add 406, that hand the buffers back at once 333
+// and 570 cycles.  Measured and not kept: half buffers of N = 128 (452 us) and tiles of
+// one weight tile with four buffers (506), both bound by the readers' fixed cost per
+// wait; scales through shared memory (427); paired multiply-adds (fma.f32x2, 561: their
+// register pairs spill).  A release of cluster scope on the arrivals cost a memory
+// barrier each (939 against 598 us at the time), issuing copies and MMAs outside uniform
+// code another third.
 
-constexpr int kBigStages = 6;
 constexpr int kBigThreads = 384;
 // Registers: 384 threads start with 168 each (64512); the first four warps drop
 // to 24 and the eight readers rise to 240 (128 * 24 + 256 * 240 = 64512).
 constexpr int kBigRegsFew = 24, kBigRegsMany = 240;
 constexpr int kBigTokens = 256;
 
+template <bool kPair>
 struct Big {
-  static constexpr int kStageBytes = 2 * kFp8TileBytes;    // 128 tokens, one weight image
-  static constexpr int kStage = kBigStages * kStageBytes;  // output staging: 4 KB per reader warp
+  static constexpr int kStages = kPair ? 6 : 4;
+  static constexpr int kStageBytes = (kPair ? 2 : 3) * kFp8TileBytes;  // 128 tokens, one or both weight images
+  static constexpr int kStage = kStages * kStageBytes;     // output staging: 4 KB per reader warp
   static constexpr int kMax = kStage + 8 * 4096;           // SwiGLU: group maxima [2][128]
   static constexpr int kBars = kMax + 1024;
-  static constexpr int kMisc = kBars + (2 * kBigStages + 4 + 1) * 8;
+  static constexpr int kMisc = kBars + (2 * kStages + 4 + 1) * 8;
   static constexpr int kTotal = kMisc + 16;
   static constexpr size_t kDynamic = (size_t)kTotal + 1024;
   static_assert(kDynamic <= 227 * 1024, "one CTA per SM");
 };
 
-// How the tiles are dealt out.  Tiles [0, whole) go round robin to the pairs of the
+// How the tiles are dealt out to pairs (or single CTAs).  Tiles [0, whole) go round robin to the
 // grid, each over all column blocks.  Each of the `rest` tiles, fewer than a full
 // round, is cut along the column blocks into `parts` pieces for as many pairs: pair
 // p's sums go to partial slot p as f32 [256 columns][256 tokens], and k_fp8_join adds
@@ -712,21 +720,23 @@ struct BigSplit {
   int whole, rest, parts;
 };
 
-// The tiles of one pair, in order: tile, column blocks [b0, b1), partial slot (or
+// The tiles of one pair or CTA, in order: tile, column blocks [b0, b1), partial slot (or
 // -1: the whole tile).  What does not change stays in the kernel's arguments.
+template <bool kPair>
 struct BigWalk {
+  static constexpr int kCtas = kPair ? 2 : 1;
   int tile, b0, b1, slot, at;
-  __device__ __forceinline__ BigWalk() : at((int)blockIdx.x / 2) {}
+  __device__ __forceinline__ BigWalk() : at((int)blockIdx.x / kCtas) {}
   __device__ __forceinline__ bool next(const BigSplit& s, int kb) {
     b0 = 0;
     b1 = kb;
     slot = -1;
     tile = at;
     if (at < s.whole) {
-      at += (int)gridDim.x / 2;
+      at += (int)gridDim.x / kCtas;
       return true;
     }
-    const int pair = (int)blockIdx.x / 2;
+    const int pair = (int)blockIdx.x / kCtas;
     if (at == INT_MAX || pair >= s.rest * s.parts) return false;
     at = INT_MAX;
     const int piece = pair % s.parts;
@@ -764,42 +774,49 @@ __device__ __forceinline__ void load_scales4(const float* row, int b, int kb, bo
   }
 }
 
-template <bool kGlu>
-__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kBigThreads, 1) k_fp8_big(const __grid_constant__ BigArgs p) {
+template <bool kGlu, bool kPair>
+__global__ void __cluster_dims__(kPair ? 2 : 1, 1, 1) __launch_bounds__(kBigThreads, 1)
+    k_fp8_big(const __grid_constant__ BigArgs p) {
+  using L = Big<kPair>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint64_t* full = reinterpret_cast<uint64_t*>(smem + Big::kBars);  // the leader's are used
-  uint64_t* empty = full + kBigStages;
-  uint64_t* d_full = empty + kBigStages;
+  uint64_t* full = reinterpret_cast<uint64_t*>(smem + L::kBars);  // the leader's are used
+  uint64_t* empty = full + L::kStages;
+  uint64_t* d_full = empty + L::kStages;
   uint64_t* d_empty = d_full + 2;  // the leader's are used
   uint64_t* drained = d_empty + 2;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + Big::kMisc);
-  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + Big::kMisc + 4);
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(smem + L::kMisc);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(smem + L::kMisc + 4);
   const MatmulArgs& g = p.g;
 
   const int warp = warp_index(), lane = threadIdx.x & 31;
-  const int rank = (int)cluster_ctarank();
+  const int rank = kPair ? (int)cluster_ctarank() : 0;
   const int mt = (int)((g.m + kBigTokens - 1) / kBigTokens), nt = (int)g.nt, kb = (int)g.kb;
-  BigWalk walk;
+  BigWalk<kPair> walk;
 
   if (threadIdx.x == 0) {
-    for (int i = 0; i < kBigStages; ++i) {
+    for (int i = 0; i < L::kStages; ++i) {
       mbar_init(&full[i], 1);
       mbar_init(&empty[i], 1);
     }
     for (int i = 0; i < 2; ++i) {
       mbar_init(&d_full[i], 1);
-      mbar_init(&d_empty[i], 16);  // eight reader warps in each CTA
+      mbar_init(&d_empty[i], kPair ? 16 : 8);  // eight reader warps in each CTA
     }
     mbar_init(drained, 1);
     *abort_flag = 0;
     fence_mbar_init();
   }
-  if (warp == 1) tmem_alloc_pair(tmem_slot, 512);
+  if (warp == 1) {
+    if constexpr (kPair) tmem_alloc_pair(tmem_slot, 512);
+    else tmem_alloc(tmem_slot, 512);
+  }
   tc_fence_before();
   __syncthreads();
-  cluster_arrive();
-  cluster_wait();
+  if constexpr (kPair) {
+    cluster_arrive();
+    cluster_wait();
+  }
   tc_fence_after();
   pdl_launch_dependents();  // after the allocation, as in k_fp8_small
   const uint32_t tmem = *tmem_slot;
@@ -810,14 +827,21 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kBigThreads, 1) k_fp
       const bool elected = elect_one();
       // a stage's copies land in both CTAs and complete on the leader's barrier
       const uint32_t full0 = mapa_shared(smem_u32(full), 0), st0 = smem_u32(smem);
+      auto load = [&](uint32_t dst, const CUtensorMap* map, int x, int y, int s) {
+        if constexpr (kPair) tma_load_2d_pair(dst, map, x, y, full0 + s * 8);
+        else tma_load_2d(smem + (dst - st0), map, x, y, &full[s]);
+      };
       auto weights = [&](int s, int unit, int b) {
-        if (rank == 0) mbar_arrive_expect_tx(&full[s], 2 * Big::kStageBytes);
-        const int t = min(unit * 2 + rank, nt - 1);  // past an odd last tile: read again, not stored
-        tma_load_2d_pair(st0 + s * Big::kStageBytes + kFp8TileBytes, &p.tm_w, 0,
-                         (int)fp8_image(g.gate_up, kb, t, b) * kFp8Group, full0 + s * 8);
+        if (rank == 0) mbar_arrive_expect_tx(&full[s], (kPair ? 2 : 1) * L::kStageBytes);
+        const uint32_t dst = st0 + s * L::kStageBytes + kFp8TileBytes;
+#pragma unroll
+        for (int i = 0; i < (kPair ? 1 : 2); ++i) {
+          const int t = min(unit * 2 + rank + i, nt - 1);  // past an odd last tile: read again, not stored
+          load(dst + i * kFp8TileBytes, &p.tm_w, 0, (int)fp8_image(g.gate_up, kb, t, b) * kFp8Group, s);
+        }
       };
       bool more = walk.next(p.split, kb);
-      int left = more ? min(walk.b1 - walk.b0, kBigStages) : 0;  // blocks whose weights are under way
+      int left = more ? min(walk.b1 - walk.b0, L::kStages) : 0;  // blocks whose weights are under way
       if (elected)
         for (int i = 0; i < left; ++i) weights(i, walk.tile / mt, walk.b0 + i);
       pdl_wait();  // the tokens come from the preceding grid
@@ -829,21 +853,25 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kBigThreads, 1) k_fp
           wait_bar(&empty[s], ph, p.err, abort_flag);
           if (elected) {
             if (left <= 0) weights(s, unit, b);
-            tma_load_2d_pair(st0 + s * Big::kStageBytes, &p.tm_a, b * kFp8Group, row, full0 + s * 8);
+            load(st0 + s * L::kStageBytes, &p.tm_a, b * kFp8Group, row, s);
           }
           --left;
-          if (++s == kBigStages) {
+          if (++s == L::kStages) {
             s = 0;
             ph ^= 1;
           }
         }
       }
       if (*abort_flag && rank == 0)  // the copies in flight land before the pair can exit
-        for (int i = 0; i < kBigStages; ++i)
+        for (int i = 0; i < L::kStages; ++i)
           mbar_wait_bounded(&full[i], i < s ? ph ^ 1 : ph, p.err, AH_ETIMEOUT, 1u << 12);
     } else if (warp == 1 && rank == 0) {
       const bool elected = elect_one();
-      constexpr uint32_t idesc = idesc_e4m3(256, 256);
+      constexpr uint32_t idesc = idesc_e4m3(kPair ? 256 : 128, 256);
+      auto commit = [](uint64_t* bar) {
+        if constexpr (kPair) mma_commit_pair(bar);
+        else mma_commit(bar);
+      };
       int s = 0, buf = 0;
       uint32_t ph = 0, dph = 1;  // the buffers start empty
       while (walk.next(p.split, kb))
@@ -851,15 +879,18 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kBigThreads, 1) k_fp
           wait_bar(&full[s], ph, p.err, abort_flag);
           wait_bar(&d_empty[buf], dph, p.err, abort_flag);
           tc_fence_after();
-          const uint32_t st = smem_u32(smem + s * Big::kStageBytes);
+          const uint32_t st = smem_u32(smem + s * L::kStageBytes);
           const uint64_t adesc = sw128_desc(st), bdesc = sw128_desc(st + kFp8TileBytes);
           if (elected) {
 #pragma unroll
-            for (int kk = 0; kk < 4; ++kk) mma_f8_pair(tmem + buf * 256, adesc + kk * 2, bdesc + kk * 2, idesc, kk > 0);
-            mma_commit_pair(&d_full[buf]);
-            mma_commit_pair(&empty[s]);
+            for (int kk = 0; kk < 4; ++kk) {
+              if constexpr (kPair) mma_f8_pair(tmem + buf * 256, adesc + kk * 2, bdesc + kk * 2, idesc, kk > 0);
+              else mma_f8(tmem + buf * 256, adesc + kk * 2, bdesc + kk * 2, idesc, kk > 0);
+            }
+            commit(&d_full[buf]);
+            commit(&empty[s]);
           }
-          if (++s == kBigStages) {
+          if (++s == L::kStages) {
             s = 0;
             ph ^= 1;
           }
@@ -867,18 +898,18 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kBigThreads, 1) k_fp
           dph ^= buf == 0;
         }
       if (*abort_flag) {  // the MMAs in flight end before the tensor memory is freed
-        if (elected) mma_commit_pair(drained);
+        if (elected) commit(drained);
         mbar_wait_bounded(drained, 0, p.err, AH_ETIMEOUT, kWaitLimit);
       }
     }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kBigRegsMany));
     const int q = warp & 3, h = (warp - 4) >> 2;  // TMEM lane quarter, column half
-    const uint32_t d_empty0 = mapa_shared(smem_u32(d_empty), 0);
+    const uint32_t d_empty0 = kPair ? mapa_shared(smem_u32(d_empty), 0) : smem_u32(d_empty);
     const uint32_t lane_addr = tmem + ((uint32_t)(q * 32) << 16) + h * 64;
     const bool vec = (reinterpret_cast<uintptr_t>(g.ascales) & 15) == 0 && g.lds % 4 == 0;
     const bool wvec = kb % 4 == 0;  // rows of scales start at multiples of 16 bytes
-    uint8_t* stage = smem + Big::kStage + (warp - 4) * 4096;
+    uint8_t* stage = smem + L::kStage + (warp - 4) * 4096;
     pdl_wait();  // the scales come from the preceding grid
     int buf = 0;
     uint32_t ph = 0;
@@ -921,7 +952,10 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kBigThreads, 1) k_fp
             } else {
               tc_fence_before();
               __syncwarp();
-              if (lane == 0) mbar_arrive_cluster(d_empty0 + buf * 8);
+              if (lane == 0) {
+                if constexpr (kPair) mbar_arrive_cluster(d_empty0 + buf * 8);
+                else mbar_arrive(&d_empty[buf]);
+              }
             }
             const float f = c < 2 ? s0[i] : s1[i];
 #pragma unroll
@@ -957,7 +991,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kBigThreads, 1) k_fp
           fm = max_abs3(fm, acc[0][j], acc[0][j + 1]);
         }
         uint32_t mx = __float_as_uint(fm);  // a NaN's bits are above every number's
-        uint32_t* maxima = reinterpret_cast<uint32_t*>(smem + Big::kMax);
+        uint32_t* maxima = reinterpret_cast<uint32_t*>(smem + L::kMax);
         maxima[h * 128 + q * 32 + lane] = mx;
         asm volatile("bar.sync 1, 256;" ::: "memory");
         mx = max(mx, maxima[(h ^ 1) * 128 + q * 32 + lane]);
@@ -1050,11 +1084,14 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(kBigThreads, 1) k_fp
 
   __syncwarp();
   __syncthreads();
-  cluster_arrive();
-  cluster_wait();
+  if constexpr (kPair) {
+    cluster_arrive();
+    cluster_wait();
+  }
   if (warp == 1) {
     tc_fence_after();
-    tmem_dealloc_pair(tmem, 512);
+    if constexpr (kPair) tmem_dealloc_pair(tmem, 512);
+    else tmem_dealloc(tmem, 512);
   }
 }
 
@@ -1140,15 +1177,18 @@ int check_device(const char* who, const AhFp8Weight* w) {
 // the last full round saves column blocks' time (about 0.45 us each) and costs a
 // launch (3 us) and the partial sums' way to L2 and back (about 6 TB/s).
 struct BigPlan {
-  int pairs;
+  bool pair;     // CTA pairs of 256 tokens, or single CTAs of 128
+  int pairs;     // pairs, or CTAs
   BigSplit split;
   size_t bytes;  // partial sums
 };
 
 BigPlan big_plan(const AhFp8Weight* w, int64_t m) {
-  const int64_t tiles = (m + kBigTokens - 1) / kBigTokens * ((w->nt + 1) / 2), pairs = std::max(1, sm_count() / 2);
+  const int64_t tiles = (m + kBigTokens - 1) / kBigTokens * ((w->nt + 1) / 2);
+  const bool pair = m > kBigTokens / 2;
+  const int64_t pairs = pair ? std::max(1, sm_count() / 2) : sm_count();
   const int64_t rest = tiles % pairs, kb = w->kb;
-  BigPlan p{(int)std::min(tiles, pairs), {(int)tiles, 0, 0}, 0};
+  BigPlan p{pair, (int)std::min(tiles, pairs), {(int)tiles, 0, 0}, 0};
   const int64_t parts = rest ? std::min<int64_t>(pairs / rest, kb / 2) : 0;  // two column blocks each at least
   if (parts < 2) return p;
   const double saved = 0.45e-6 * (double)(kb - (kb + parts - 1) / parts);
@@ -1160,7 +1200,7 @@ BigPlan big_plan(const AhFp8Weight* w, int64_t m) {
   return p;
 }
 
-template <bool kGlu>
+template <bool kGlu, bool kPair>
 int launch_big(BigArgs& p, const BigPlan& plan, cudaStream_t st) {
   const MatmulArgs& g = p.g;
   int rc = encode_rows(&p.tm_a, g.a, (uint64_t)g.cols, (uint64_t)g.m, (uint64_t)g.lda, 128);
@@ -1187,9 +1227,9 @@ int launch_big(BigArgs& p, const BigPlan& plan, cudaStream_t st) {
   if (rc != AH_OK) return rc;
   static int regs[64];
   std::call_once(once[dev], [&] {
-    attr[dev] = cudaFuncSetAttribute(k_fp8_big<kGlu>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Big::kDynamic);
+    attr[dev] = cudaFuncSetAttribute(k_fp8_big<kGlu, kPair>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)Big<kPair>::kDynamic);
     cudaFuncAttributes a{};
-    if (attr[dev] == cudaSuccess) attr[dev] = cudaFuncGetAttributes(&a, k_fp8_big<kGlu>);
+    if (attr[dev] == cudaSuccess) attr[dev] = cudaFuncGetAttributes(&a, k_fp8_big<kGlu, kPair>);
     regs[dev] = a.numRegs;
   });
   AH_CUDA_TRY(attr[dev]);
@@ -1197,21 +1237,23 @@ int launch_big(BigArgs& p, const BigPlan& plan, cudaStream_t st) {
   if (regs[dev] * kBigThreads < kBigRegsFew * 128 + kBigRegsMany * 256)
     return fail(AH_EUNSUPPORTED, "fp8w_matmul: built with %d registers per thread, too few to redistribute", regs[dev]);
   p.split = plan.split;
-  rc = launch_pdl(k_fp8_big<kGlu>, dim3((unsigned)(2 * plan.pairs)), dim3(kBigThreads), Big::kDynamic, st,
+  rc = launch_pdl(k_fp8_big<kGlu, kPair>, dim3((unsigned)((kPair ? 2 : 1) * plan.pairs)), dim3(kBigThreads), Big<kPair>::kDynamic, st,
                   (const BigArgs)p);
   if (rc != AH_OK || plan.split.rest == 0) return rc;
   const unsigned chunks = (unsigned)std::min<int64_t>(kBigTokens / 32, (g.m + 31) / 32);
   return launch_pdl(k_fp8_join<kGlu>, dim3(chunks, (unsigned)plan.split.rest), dim3(kJoinThreads), 0, st, (const BigArgs)p);
 }
 
-// Whether a product goes to the pair kernel.  The weight-streaming kernel takes up
-// to 64 tokens (14336 x 4096 at 64 tokens: 16.4 us against 19.6, a 4096 x 14336
-// feed-forward block 51 against 63), and more while its tiles, one per 64 tokens (32
-// for a gate/up pair), leave clusters of four (two) on two CTAs per SM: 4096 x 4096
-// at 128 tokens 10.6 us against 13.3, but at 192 15.0 against 13.7, and 8192 x 512 at
-// 128 7.2 against 6.1.
+// Whether a product goes to k_fp8_big.  The weight-streaming kernel
+// takes up to 32, and 33 to 64 while the tiles of single CTAs would leave a third of the
+// SMs idle (64 tokens: 14336 x 4096 17.7 us against 19.0, but 28672 x 8192 49 against
+// 43, a 4096 x 14336 feed-forward block 50 with its gate/up product there against 44).  It takes more while its tiles, one per 64 tokens (32 for a gate/up pair), leave
+// clusters of four (two) on two CTAs per SM: 4096 x 4096 at 128 tokens 12.0 us against
+// 16.1 of single CTAs, but at 192 15.0 against 13.7 of pairs, and 8192 x 512 at 128 7.2
+// against 6.1.
 bool use_big(const AhFp8Weight* w, bool glu, int64_t m) {
-  if (m <= 64) return false;
+  if (m <= 32) return false;
+  if (m <= 64) return (w->nt + 1) / 2 * 3 > sm_count() * 2;
   return glu ? w->nt / 2 * ((m + 31) / 32) > sm_count() : w->nt * ((m + 63) / 64) > sm_count() / 2;
 }
 
@@ -1234,7 +1276,7 @@ int run_matmul(const MatmulArgs& g, const AhFp8Weight* w, float* partial, size_t
     AH_REQUIRE(!partial || bytes >= plan.bytes, "fp8w_matmul: workspace of %zu bytes, %zu needed", bytes, plan.bytes);
     if (plan.split.rest && !partial) {  // no workspace: no split
       const int64_t tiles = plan.split.whole + plan.split.rest;
-      plan.pairs = (int)std::min<int64_t>(tiles, std::max(1, sm_count() / 2));
+      plan.pairs = (int)std::min<int64_t>(tiles, plan.pair ? std::max(1, sm_count() / 2) : sm_count());
       plan.split = BigSplit{(int)tiles, 0, 0};
     }
     BigArgs p{};
@@ -1242,7 +1284,7 @@ int run_matmul(const MatmulArgs& g, const AhFp8Weight* w, float* partial, size_t
     p.partial = partial;
     p.err = device_error_word();
     set(p);
-    return launch_big<kGlu>(p, plan, st);
+    return plan.pair ? launch_big<kGlu, true>(p, plan, st) : launch_big<kGlu, false>(p, plan, st);
   }
   SmallArgs p{};
   p.g = g;

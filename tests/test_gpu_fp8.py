@@ -264,6 +264,11 @@ LARGE = [(129, 5000, 130), (300, 4000, 200), (256, 5120, 128), (257, 2433, 1), (
          (1025, 1152, 520), (2100, 1003, 257), (4100, 640, 96)]
 
 
+# 33 to 128 tokens: one tile of single CTAs, several tiles each, odd numbers of weight
+# tiles, tiles split along K, outputs a tensor map can and cannot address
+LARGE += [(33, 25500, 160), (64, 38800, 300), (48, 40960, 1280), (65, 20000, 130), (128, 10240, 384), (127, 40100, 300), (96, 9601, 2048), (100, 4864, 1280), (128, 80000, 96)]
+
+
 @pytest.mark.parametrize("m,n,k", LARGE)
 def test_matmul_large(fp8, m, n, k):
     wq, ws = blocks(n, k, m + n + k)
@@ -440,6 +445,7 @@ def ffn_weights(n_embd, n_ff, seed):
 
 FFN = [(1, 256, 384), (1, 1024, 2048), (3, 130, 200), (16, 512, 700), (40, 200, 1000), (130, 384, 512),
        (300, 640, 1030), (600, 256, 300), (320, 8192, 2000), (520, 300, 2200)]
+FFN += [(50, 256, 12900), (100, 300, 13000), (128, 256, 19500)]  # gate/up tiles of single CTAs, whole and split
 
 
 @pytest.mark.parametrize("m,n_embd,n_ff", FFN)
