@@ -158,6 +158,8 @@ int build(const TileSource (&s)[2], int kind, bool gate_up, int64_t rows, int64_
     AH_REQUIRE(s[i].p && s[i].ld >= cols, "fp8w: null source or a row stride below cols");
     AH_REQUIRE(kind != kSourceE4m3 || (s[i].scales && s[i].lds >= fp8_groups(cols)),
                "fp8w: null scales or a scale row stride below ceil(cols / 128)");
+    AH_REQUIRE(kind == kSourceE4m3 ? element_aligned(s[i].scales, AH_DTYPE_F32) : element_aligned(s[i].p, kind == kSourceF32 ? AH_DTYPE_F32 : AH_DTYPE_F16),
+               "fp8w: a source is not aligned to its elements");
   }
   AhFp8Weight* w = new (std::nothrow) AhFp8Weight();
   if (!w) return fail(AH_ENOMEM, "fp8w: out of host memory");
@@ -1304,6 +1306,8 @@ int matmul(const AhFp8Weight* w, const uint8_t* q, int64_t ldq, const float* sca
   AH_REQUIRE(aligned16(q) && ldq % 16 == 0 && ldq >= w->cols,
              "fp8w_matmul: q rows must start at multiples of 16 bytes, ldq >= cols");
   AH_REQUIRE(lds >= w->kb && ldy >= w->rows, "fp8w_matmul: lds below ceil(cols / 128) or ldy below rows");
+  AH_REQUIRE(element_aligned(scales, AH_DTYPE_F32) && element_aligned(y, y_dtype),
+             "fp8w_matmul: scales or y are not aligned to their elements");
   AH_REQUIRE(aligned16(workspace), "fp8w_matmul: the workspace must be 16-byte aligned");
   rc = check_device("fp8w_matmul", w);
   if (rc != AH_OK) return rc;
@@ -1355,6 +1359,7 @@ int check_ffn(const AhFp8Weight* gate_up, const AhFp8Weight* down, int64_t m) {
   AH_REQUIRE(gate_up && down, "fp8_ffn: null weight");
   AH_REQUIRE(gate_up->gate_up && !down->gate_up && down->cols == gate_up->rows / 2 && down->rows == gate_up->cols,
              "fp8_ffn: needs a gate/up weight of 2 * n_ff rows and a down weight [n_embd][n_ff]");
+  AH_REQUIRE(gate_up->nt / 2 <= 65535 && down->nt <= 65535, "fp8_ffn: more than 65535 row tiles");
   const int rc = check_matmul(gate_up, m);
   return rc != AH_OK ? rc : check_matmul(down, m);
 }
@@ -1438,6 +1443,7 @@ int ah_fp8_ffn(const AhFp8Weight* gate_up, const AhFp8Weight* down, const void* 
   AH_REQUIRE(y && ldy >= down->rows, "fp8_ffn: null y or ldy below n_embd");
   AH_REQUIRE(y_dtype == AH_DTYPE_F32 || y_dtype == AH_DTYPE_F16 || y_dtype == AH_DTYPE_BF16,
              "fp8_ffn: output dtype %u is not f32, f16 or bf16", y_dtype);
+  AH_REQUIRE(element_aligned(y, y_dtype), "fp8_ffn: y is not aligned to its elements");
   const FfnLayout l = ffn_layout(gate_up, down, m);
   AH_REQUIRE(workspace && aligned16(workspace), "fp8_ffn: the workspace must be 16-byte aligned");
   AH_REQUIRE(workspace_bytes >= l.total, "fp8_ffn: workspace of %zu bytes, %zu needed", workspace_bytes, l.total);

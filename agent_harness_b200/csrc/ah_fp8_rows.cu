@@ -403,6 +403,7 @@ int check_rows(const char* who, int64_t m, int64_t k, const void* q, int64_t ldq
   AH_REQUIRE(aligned16(q) && ldq % 16 == 0 && ldq >= k, "%s: q rows must start at multiples of 16 bytes, ldq >= k",
              who);
   AH_REQUIRE(lds >= fp8_groups(k), "%s: lds must be at least ceil(k / 128)", who);
+  AH_REQUIRE(element_aligned(scales, AH_DTYPE_F32), "%s: scales are not aligned to their elements", who);
   return AH_OK;
 }
 
@@ -482,6 +483,7 @@ int ah_fp8_quantize(const void* x, int64_t ldx, uint32_t dtype, int64_t m, int64
   const int rc = check_rows("fp8_quantize", m, k, q, ldq, scales, lds, dtype);
   if (rc != AH_OK || m == 0) return rc;
   AH_REQUIRE(x && ldx >= k, "fp8_quantize: null x or ldx below k");
+  AH_REQUIRE(element_aligned(x, dtype), "fp8_quantize: x is not aligned to its elements");
   const RowArgs g{x, nullptr, ldx, 0, m, (int)k, q, ldq, scales, lds};
   return dispatch_rows<kRowQuantize>(g, dtype, vec_rows(x, ldx, dtype), as_stream(stream));
 }
@@ -491,6 +493,8 @@ int ah_fp8_swiglu(const void* gate, int64_t ld_gate, const void* up, int64_t ld_
   const int rc = check_rows("fp8_swiglu", m, k, q, ldq, scales, lds, dtype);
   if (rc != AH_OK || m == 0) return rc;
   AH_REQUIRE(gate && up && ld_gate >= k && ld_up >= k, "fp8_swiglu: null input or a row stride below k");
+  AH_REQUIRE(element_aligned(gate, dtype) && element_aligned(up, dtype),
+             "fp8_swiglu: an input is not aligned to its elements");
   const RowArgs g{gate, up, ld_gate, ld_up, m, (int)k, q, ldq, scales, lds};
   return dispatch_rows<kRowSwiglu>(g, dtype, vec_rows(gate, ld_gate, dtype) && vec_rows(up, ld_up, dtype),
                                    as_stream(stream));
@@ -505,6 +509,8 @@ int ah_fp8_add_rms_norm(const void* x, int64_t ldx, void* residual, int64_t ldr,
   AH_REQUIRE(!residual || ldr >= k, "fp8_add_rms_norm: ldr below k");
   AH_REQUIRE(norm_dtype == AH_DTYPE_F32 || norm_dtype == AH_DTYPE_F16 || norm_dtype == AH_DTYPE_BF16,
              "fp8_add_rms_norm: norm weight dtype %u is not f32, f16 or bf16", norm_dtype);
+  AH_REQUIRE(element_aligned(x, dtype) && element_aligned(residual, dtype) && element_aligned(norm_w, norm_dtype),
+             "fp8_add_rms_norm: an input is not aligned to its elements");
   AH_REQUIRE(eps >= 0.0f, "fp8_add_rms_norm: eps must be >= 0");
   const NormArgs g{x, residual, norm_w, ldx, ldr, m, (int)k, q, ldq, scales, lds, norm_dtype, aligned16(norm_w), eps};
   const bool vec = vec_rows(x, ldx, dtype) && (!residual || vec_rows(residual, ldr, dtype)) && g.w_aligned;

@@ -43,6 +43,15 @@ def test_entry_specific_refusals(entry, fault):
     assert entry(**fault) == EINVAL
 
 
+@pytest.mark.parametrize("entry,fault", [
+    (quantize, dict(x=P + 2)), (quantize, dict(x=P + 1, dt=1)), (quantize, dict(s=P + 2)), (swiglu, dict(g=P + 1)),
+    (swiglu, dict(u=P + 3)), (norm, dict(x=P + 1)), (norm, dict(r=P + 1)), (norm, dict(w=P + 1)),
+    (norm, dict(w=P + 2, wdt=0))])
+def test_pointers_off_their_elements_are_refused(entry, fault):
+    assert entry(**fault) == EINVAL
+    assert b"aligned to" in lib().ah_last_error()
+
+
 @pytest.mark.parametrize("entry", [quantize, swiglu, norm])
 def test_no_rows_is_a_no_op(entry):
     assert entry(m=0) == OK
@@ -60,6 +69,14 @@ def test_weight_makers_refuse():
     assert L.ah_fp8w_quantize(P, 199, 0, 100, 200, C.byref(h), None) == EINVAL
     assert L.ah_fp8w_from_blocks_gate_up(P, 200, P, 2, 0, 200, P, 2, 100, 200, C.byref(h), None) == EINVAL
     assert L.ah_fp8w_quantize_gate_up(P, 200, P, 199, 0, 100, 200, C.byref(h), None) == EINVAL
+
+
+def test_weight_makers_refuse_sources_off_their_elements():
+    h = C.c_void_p()
+    L = lib()
+    assert L.ah_fp8w_from_blocks(P, 200, P + 2, 2, 100, 200, C.byref(h), None) == EINVAL
+    assert L.ah_fp8w_quantize(P + 2, 200, 0, 100, 200, C.byref(h), None) == EINVAL
+    assert L.ah_fp8w_quantize_gate_up(P, 200, P + 1, 200, 1, 100, 200, C.byref(h), None) == EINVAL
 
 
 def test_null_weights_refused():
