@@ -259,6 +259,26 @@ __device__ __forceinline__ void store_y4(void* y, int64_t at, uint32_t dtype, co
     if (i < n) store_y(y, at + i, dtype, v[i]);
 }
 
+// SwiGLU and quantise of one token's group `unit`, four columns per lane, by a warp:
+// p.act_q, p.act_scales.  rows = n_ff.
+template <typename Args>
+__device__ __forceinline__ void store_swiglu4(const Args& p, int64_t token, int64_t unit, int64_t rows,
+                                              const float (&gate)[4], const float (&up)[4]) {
+  const int lane = threadIdx.x & 31;
+  const int64_t r = unit * kFp8Group + lane * 4;
+  float o[4];
+#pragma unroll
+  for (int i = 0; i < 4; ++i) o[i] = r + i < rows ? fp8_silu_mul(gate[i], up[i]) : 0.0f;
+  const float fm = max_abs3(max_abs3(kFp8Tiny, o[0], o[1]), o[2], o[3]);
+  const float gm = __uint_as_float(__reduce_max_sync(0xFFFFFFFFu, __float_as_uint(fm))), inv = fp8_inverse(gm);
+  const uint32_t w = cvt_e4m3x4(o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv);
+  uint8_t* qrow = p.act_q + token * p.ld_act + r;  // ld_act is a multiple of 16
+  if (r + 4 <= rows) *reinterpret_cast<uint32_t*>(qrow) = w;
+  else
+    for (int i = 0; i < 4 && r + i < rows; ++i) qrow[i] = (uint8_t)(w >> (8 * i));
+  if (lane == 0) p.act_scales[token * p.lds_act + unit] = gm * (1.0f / kFp8Max);
+}
+
 // ---- few tokens: weight rows on the MMA's M, tokens on N ------------------------------
 //
 // A CTA takes one 128-row tile (or a gate/up pair of tiles) and a run of its
@@ -581,16 +601,7 @@ __global__ void __launch_bounds__(kSmallThreads, 2) k_fp8_small(const __grid_con
       if constexpr (kGlu) {
         float up[4];
         sum4(kNt + c, up);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) o[i] = r + i < rows ? fp8_silu_mul(o[i], up[i]) : 0.0f;
-        const float fm = max_abs3(max_abs3(kFp8Tiny, o[0], o[1]), o[2], o[3]);
-        const float gm = __uint_as_float(__reduce_max_sync(0xFFFFFFFFu, __float_as_uint(fm))), inv = fp8_inverse(gm);
-        const uint32_t w = cvt_e4m3x4(o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv);
-        uint8_t* qrow = p.act_q + (m0 + c) * p.ld_act + r;  // ld_act is a multiple of 16
-        if (r + 4 <= rows) *reinterpret_cast<uint32_t*>(qrow) = w;
-        else
-          for (int i = 0; i < 4 && r + i < rows; ++i) qrow[i] = (uint8_t)(w >> (8 * i));
-        if (lane == 0) p.act_scales[(m0 + c) * p.lds_act + unit] = gm * (1.0f / kFp8Max);
+        store_swiglu4(p, m0 + c, unit, rows, o, up);
       } else {
         const int64_t at = (m0 + c) * g.ldy + (g.gate_up && (unit & 1) ? rows : 0) + r;
         store_y4(g.y, at, g.y_dtype, o, (int)min((int64_t)4, rows - r));
@@ -678,7 +689,11 @@ int dispatch_small(SmallArgs& p, cudaStream_t st) {
 //
 // Up to 128 tokens (!kPair) single CTAs walk tiles of 128 tokens x two weight tiles,
 // loading both images (48 KB per column block, M = 128): half of a pair's rows would be
-// empty.  128 x 28672 x 8192 45 us (5.2 TB/s of weights; pairs 66), 128 x 32000 x 2048
+// empty.  A tile's column blocks are shared by a cluster of two, four or eight where
+// that many fit the GPU at once; its members add their sums through distributed shared
+// memory in rank order (65 x 6144 x 4096 12.7 us, by partial sums in global memory and a
+// second launch 14.5; 65 x 8192 x 8192 19.0 against 20.8; requesting several tokens' sums
+// at a time was no faster).  128 x 28672 x 8192 45 us (5.2 TB/s of weights; pairs 66), 128 x 32000 x 2048
 // 16.7 (24), a 4096 x 14336 feed-forward block at 128 tokens 53 (65).  Past 128 tokens
 // single CTAs load half as much again: 443 us where pairs take 414.
 //
@@ -756,6 +771,7 @@ struct BigArgs {
   CUtensorMap tm_y;  // y [m][rows], box 128 bytes x 32 rows, 128-byte swizzle (when y_map)
   MatmulArgs g;
   bool y_map;
+  bool cluster;  // single CTAs: a split tile's parts are a cluster and add their sums in it
   BigSplit split;
   float* partial;
   uint8_t* act_q;
@@ -776,9 +792,45 @@ __device__ __forceinline__ void load_scales4(const float* row, int b, int kb, bo
   }
 }
 
+// One token of a tile that a cluster of nc CTAs shares: the members' sums at `at` in their
+// shared memory (four columns of weight tile 0, tile 1's 64 KB on), in rank order, by
+// one warp, and the token's output.
+template <bool kGlu>
+__device__ __forceinline__ void join_token(const BigArgs& p, int unit, int token, uint32_t at, int nc) {
+  const MatmulArgs& g = p.g;
+  const int lane = threadIdx.x & 31;
+  float o[2][4];
+#pragma unroll
+  for (int t = 0; t < 2; ++t) {
+    uint4 v[kMaxCluster];
+#pragma unroll
+    for (int k = 0; k < kMaxCluster; ++k)
+      if (k < nc) v[k] = ld_dsmem_v4(mapa_shared(at + t * 65536, k));
+    o[t][0] = o[t][1] = o[t][2] = o[t][3] = 0.0f;
+#pragma unroll
+    for (int k = 0; k < kMaxCluster; ++k)
+      if (k < nc) {
+        o[t][0] += __uint_as_float(v[k].x);
+        o[t][1] += __uint_as_float(v[k].y);
+        o[t][2] += __uint_as_float(v[k].z);
+        o[t][3] += __uint_as_float(v[k].w);
+      }
+  }
+  const int64_t rows = g.gate_up ? g.rows / 2 : g.rows;  // rows of a tile's source
+  if constexpr (kGlu) {
+    store_swiglu4(p, token, unit, rows, o[0], o[1]);
+  } else {
+#pragma unroll
+    for (int t = 0; t < 2; ++t) {
+      const int64_t r = (int64_t)(g.gate_up ? unit : unit * 2 + t) * kFp8Group + lane * 4;
+      store_y4(g.y, (int64_t)token * g.ldy + (g.gate_up ? t * rows : 0) + r, g.y_dtype, o[t],
+               (int)max((int64_t)0, min((int64_t)4, rows - r)));
+    }
+  }
+}
+
 template <bool kGlu, bool kPair>
-__global__ void __cluster_dims__(kPair ? 2 : 1, 1, 1) __launch_bounds__(kBigThreads, 1)
-    k_fp8_big(const __grid_constant__ BigArgs p) {
+__global__ void __launch_bounds__(kBigThreads, 1) k_fp8_big(const __grid_constant__ BigArgs p) {
   using L = Big<kPair>;
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
@@ -904,6 +956,11 @@ __global__ void __cluster_dims__(kPair ? 2 : 1, 1, 1) __launch_bounds__(kBigThre
         mbar_wait_bounded(drained, 0, p.err, AH_ETIMEOUT, kWaitLimit);
       }
     }
+    if (!kPair && p.cluster) {  // the readers' exchange
+      __syncwarp();
+      cluster_arrive();
+      cluster_wait();
+    }
   } else {
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kBigRegsMany));
     const int q = warp & 3, h = (warp - 4) >> 2;  // TMEM lane quarter, column half
@@ -971,6 +1028,21 @@ __global__ void __cluster_dims__(kPair ? 2 : 1, 1, 1) __launch_bounds__(kBigThre
         }
       }
       const bool ok = !__any_sync(0xFFFFFFFFu, *abort_flag);  // after a give-up nothing is stored
+      if (!kPair && walk.slot >= 0 && p.cluster) {
+        // to the idle ring as [tile][token][128 columns], 16-byte pieces of a token's row
+        // at piece ^ (token % 32)
+        if (ok) {
+          const uint32_t row = smem_u32(smem) + (q * 32 + lane) * 512;
+#pragma unroll
+          for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int j = 0; j < 16; ++j)
+              asm volatile("st.shared.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(row + t * 65536 + (((h * 16 + j) ^ lane) << 4)),
+                           "f"(acc[t][4 * j]), "f"(acc[t][4 * j + 1]), "f"(acc[t][4 * j + 2]), "f"(acc[t][4 * j + 3])
+                           : "memory");
+        }
+        continue;
+      }
       if (walk.slot >= 0) {
         // columns 64 h + j of weight tile t at 128 t + 64 h + j: a warp stores 32 tokens
         float* out = p.partial + ((int64_t)walk.slot * 256 + h * 64) * kBigTokens + rank * 128 + q * 32 + lane;
@@ -1082,11 +1154,21 @@ __global__ void __cluster_dims__(kPair ? 2 : 1, 1, 1) __launch_bounds__(kBigThre
       }
     }
     if (lane == 0) bulk_wait_all();  // the stage is read, the stores complete
+    if (!kPair && p.cluster) {
+      __syncwarp();
+      cluster_arrive();
+      cluster_wait();
+      if (!*abort_flag) {
+        const int nc = p.split.parts;
+        for (int c = (int)cluster_ctarank() + (warp - 4) * nc; c < (int)g.m; c += 8 * nc)
+          join_token<kGlu>(p, (int)blockIdx.x / nc, c, smem_u32(smem) + c * 512 + ((lane ^ (c & 31)) << 4), nc);
+      }
+    }
   }
 
   __syncwarp();
   __syncthreads();
-  if constexpr (kPair) {
+  if (kPair || p.cluster) {  // the other CTAs are done with this one's shared memory
     cluster_arrive();
     cluster_wait();
   }
@@ -1175,22 +1257,62 @@ int check_device(const char* who, const AhFp8Weight* w) {
   return AH_OK;
 }
 
-// The pairs of a launch and how its tiles are dealt out.  Splitting the tiles past
+// The pairs (or single CTAs) of a launch and how its tiles are dealt out.  Splitting the tiles past
 // the last full round saves column blocks' time (about 0.45 us each) and costs a
 // launch (3 us) and the partial sums' way to L2 and back (about 6 TB/s).
 struct BigPlan {
   bool pair;     // CTA pairs of 256 tokens, or single CTAs of 128
+  bool cluster;  // single CTAs: tiles cut along K over clusters
   int pairs;     // pairs, or CTAs
   BigSplit split;
   size_t bytes;  // partial sums
 };
+
+// Clusters of c single CTAs that the current device holds at a time.
+int max_clusters(int c) {
+  static std::once_flag once[64];
+  static int most[64][kMaxCluster + 1];
+  int dev = 0;
+  if (cudaGetDevice(&dev) != cudaSuccess || dev < 0 || dev >= 64) return 0;
+  std::call_once(once[dev], [&] {
+    if (cudaFuncSetAttribute(k_fp8_big<false, false>, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                             (int)Big<false>::kDynamic) != cudaSuccess) {
+      cudaGetLastError();
+      return;
+    }
+    for (int n = 2; n <= kMaxCluster; n *= 2) {
+      cudaLaunchAttribute at{};
+      at.id = cudaLaunchAttributeClusterDimension;
+      at.val.clusterDim.x = (unsigned)n;
+      at.val.clusterDim.y = at.val.clusterDim.z = 1;
+      cudaLaunchConfig_t cfg{};
+      cfg.gridDim = dim3((unsigned)n);
+      cfg.blockDim = dim3(kBigThreads);
+      cfg.dynamicSmemBytes = Big<false>::kDynamic;
+      cfg.attrs = &at;
+      cfg.numAttrs = 1;
+      if (cudaOccupancyMaxActiveClusters(&most[dev][n], k_fp8_big<false, false>, &cfg) != cudaSuccess) {
+        cudaGetLastError();
+        most[dev][n] = 0;
+      }
+    }
+  });
+  return most[dev][c];
+}
 
 BigPlan big_plan(const AhFp8Weight* w, int64_t m) {
   const int64_t tiles = (m + kBigTokens - 1) / kBigTokens * ((w->nt + 1) / 2);
   const bool pair = m > kBigTokens / 2;
   const int64_t pairs = pair ? std::max(1, sm_count() / 2) : sm_count();
   const int64_t rest = tiles % pairs, kb = w->kb;
-  BigPlan p{pair, (int)std::min(tiles, pairs), {(int)tiles, 0, 0}, 0};
+  BigPlan p{pair, false, (int)std::min(tiles, pairs), {(int)tiles, 0, 0}, 0};
+  for (int c = kMaxCluster; !pair && c >= 2; c /= 2)
+    if (kb >= 4 * c && tiles <= max_clusters(c)) {  // four column blocks each at least
+      p.cluster = true;
+      p.pairs = (int)tiles * c;
+      p.split = BigSplit{0, (int)tiles, c};
+      return p;
+    }
   const int64_t parts = rest ? std::min<int64_t>(pairs / rest, kb / 2) : 0;  // two column blocks each at least
   if (parts < 2) return p;
   const double saved = 0.45e-6 * (double)(kb - (kb + parts - 1) / parts);
@@ -1239,9 +1361,23 @@ int launch_big(BigArgs& p, const BigPlan& plan, cudaStream_t st) {
   if (regs[dev] * kBigThreads < kBigRegsFew * 128 + kBigRegsMany * 256)
     return fail(AH_EUNSUPPORTED, "fp8w_matmul: built with %d registers per thread, too few to redistribute", regs[dev]);
   p.split = plan.split;
-  rc = launch_pdl(k_fp8_big<kGlu, kPair>, dim3((unsigned)((kPair ? 2 : 1) * plan.pairs)), dim3(kBigThreads), Big<kPair>::kDynamic, st,
-                  (const BigArgs)p);
-  if (rc != AH_OK || plan.split.rest == 0) return rc;
+  p.cluster = plan.cluster;
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = dim3((unsigned)((kPair ? 2 : 1) * plan.pairs));
+  cfg.blockDim = dim3(kBigThreads);
+  cfg.dynamicSmemBytes = Big<kPair>::kDynamic;
+  cfg.stream = st;
+  cudaLaunchAttribute at[2];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  at[1].id = cudaLaunchAttributeClusterDimension;
+  at[1].val.clusterDim.x = kPair ? 2 : plan.cluster ? (unsigned)plan.split.parts : 1;
+  at[1].val.clusterDim.y = 1;
+  at[1].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 2;
+  AH_CUDA_TRY(cudaLaunchKernelEx(&cfg, k_fp8_big<kGlu, kPair>, (const BigArgs)p));
+  if (plan.split.rest == 0 || plan.cluster) return AH_OK;
   const unsigned chunks = (unsigned)std::min<int64_t>(kBigTokens / 32, (g.m + 31) / 32);
   return launch_pdl(k_fp8_join<kGlu>, dim3(chunks, (unsigned)plan.split.rest), dim3(kJoinThreads), 0, st, (const BigArgs)p);
 }
@@ -1276,7 +1412,7 @@ int run_matmul(const MatmulArgs& g, const AhFp8Weight* w, float* partial, size_t
   if (use_big(w, kGlu, g.m)) {
     BigPlan plan = big_plan(w, g.m);
     AH_REQUIRE(!partial || bytes >= plan.bytes, "fp8w_matmul: workspace of %zu bytes, %zu needed", bytes, plan.bytes);
-    if (plan.split.rest && !partial) {  // no workspace: no split
+    if (plan.split.rest && !plan.cluster && !partial) {  // no workspace: no split
       const int64_t tiles = plan.split.whole + plan.split.rest;
       plan.pairs = (int)std::min<int64_t>(tiles, plan.pair ? std::max(1, sm_count() / 2) : sm_count());
       plan.split = BigSplit{(int)tiles, 0, 0};

@@ -267,6 +267,8 @@ LARGE = [(129, 5000, 130), (300, 4000, 200), (256, 5120, 128), (257, 2433, 1), (
 # 33 to 128 tokens: one tile of single CTAs, several tiles each, odd numbers of weight
 # tiles, tiles split along K, outputs a tensor map can and cannot address
 LARGE += [(33, 25500, 160), (64, 38800, 300), (48, 40960, 1280), (65, 20000, 130), (128, 10240, 384), (127, 40100, 300), (96, 9601, 2048), (100, 4864, 1280), (128, 80000, 96)]
+# tiles cut along K over clusters of two, four and eight CTAs, uneven parts
+LARGE += [(128, 15000, 1100), (65, 7900, 2100), (127, 5000, 4300), (100, 4864, 4224)]
 
 
 @pytest.mark.parametrize("m,n,k", LARGE)
@@ -280,8 +282,8 @@ def test_matmul_large(fp8, m, n, k):
 
 
 # tiles past the last full round of the GPU's pairs, cut along the columns
-SPLIT = [(260, 2048, 8192), (300, 1930, 8200), (520, 1200, 6000), (65, 5000, 16000), (2048, 9500, 3200)]
-WHOLE = [(512, 1100, 6000), (65, 4300, 16000)]  # few enough tiles for the other kernel: no workspace
+SPLIT = [(260, 2048, 8192), (300, 1930, 8200), (520, 1200, 6000), (100, 40960, 3200), (2048, 9500, 3200)]
+WHOLE = [(512, 1100, 6000), (65, 4300, 16000), (65, 5000, 16000)]  # not split, or inside clusters: no workspace
 
 
 @pytest.mark.parametrize("m,n,k", SPLIT + WHOLE)
@@ -445,7 +447,7 @@ def ffn_weights(n_embd, n_ff, seed):
 
 FFN = [(1, 256, 384), (1, 1024, 2048), (3, 130, 200), (16, 512, 700), (40, 200, 1000), (130, 384, 512),
        (300, 640, 1030), (600, 256, 300), (320, 8192, 2000), (520, 300, 2200)]
-FFN += [(50, 256, 12900), (100, 300, 13000), (128, 256, 19500)]  # gate/up tiles of single CTAs, whole and split
+FFN += [(50, 256, 12900), (100, 300, 13000), (128, 256, 19500), (80, 1100, 6500)]  # gate/up tiles of single CTAs
 
 
 @pytest.mark.parametrize("m,n_embd,n_ff", FFN)
