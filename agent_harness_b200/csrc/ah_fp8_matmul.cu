@@ -1387,7 +1387,7 @@ int launch_big(BigArgs& p, const BigPlan& plan, cudaStream_t st) {
 // SMs idle (64 tokens: 14336 x 4096 17.7 us against 19.0, but 28672 x 8192 49 against
 // 43, a 4096 x 14336 feed-forward block 50 with its gate/up product there against 44).  It takes more while its tiles, one per 64 tokens (32 for a gate/up pair), leave
 // clusters of four (two) on two CTAs per SM: 4096 x 4096 at 128 tokens 12.0 us against
-// 16.1 of single CTAs, but at 192 15.0 against 13.7 of pairs, and 8192 x 512 at 128 7.2
+// 14.2 of single CTAs, but at 192 15.0 against 13.7 of pairs, and 8192 x 512 at 128 7.2
 // against 6.1.
 bool use_big(const AhFp8Weight* w, bool glu, int64_t m) {
   if (m <= 32) return false;

@@ -606,6 +606,34 @@ def test_first_call_may_be_captured(fp8, m):
     assert r.returncode == 0, r.stdout + r.stderr
 
 
+_FRESH_PRODUCT = """
+import sys, torch
+sys.path.insert(0, sys.argv[1])
+from agent_harness_b200 import fp8
+m = int(sys.argv[2])
+W = fp8.Fp8Weight.from_float(torch.randn(8192, 2048, device="cuda"))
+q, s = fp8.quantize_fp8(torch.randn(m, 2048, device="cuda"))
+y = torch.empty(m, 8192, device="cuda")
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    W.matmul(q, s, out=y)
+graph.replay()
+for _ in range(6):
+    assert torch.equal(W.matmul(q, s), y), "captured and eager differ"
+"""
+
+
+@pytest.mark.parametrize("m", [65, 128])
+def test_first_clustered_product_may_be_captured(fp8, m):
+    """Clusters are counted on the first call, also while that is captured."""
+    import os
+    import subprocess
+    import sys
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    r = subprocess.run([sys.executable, "-c", _FRESH_PRODUCT, root, str(m)], capture_output=True, text=True, timeout=300)
+    assert r.returncode == 0, r.stdout + r.stderr
+
+
 def test_operators_on_unlike_streams(fp8):
     """Inputs made on one stream, used on another that waits for it, outputs read on a third."""
     a, b = torch.cuda.Stream(), torch.cuda.Stream()
