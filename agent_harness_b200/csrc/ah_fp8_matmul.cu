@@ -267,8 +267,9 @@ __device__ __forceinline__ void store_swiglu4(const Args& p, int64_t token, int6
   const int lane = threadIdx.x & 31;
   const int64_t r = unit * kFp8Group + lane * 4;
   float o[4];
+  fp8_silu_mul(gate, up, o);
 #pragma unroll
-  for (int i = 0; i < 4; ++i) o[i] = r + i < rows ? fp8_silu_mul(gate[i], up[i]) : 0.0f;
+  for (int i = 0; i < 4; ++i) o[i] = r + i < rows ? o[i] : 0.0f;
   const float fm = max_abs3(max_abs3(kFp8Tiny, o[0], o[1]), o[2], o[3]);
   const float gm = __uint_as_float(__reduce_max_sync(0xFFFFFFFFu, __float_as_uint(fm))), inv = fp8_inverse(gm);
   const uint32_t w = cvt_e4m3x4(o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv);
@@ -1056,14 +1057,11 @@ __global__ void __launch_bounds__(kBigThreads, 1) k_fp8_big(const __grid_constan
       }
       if constexpr (kGlu) {
         const int64_t n_ff = g.rows / 2, c0 = (int64_t)unit * kFp8Group + h * 64;
+        // rows past n_ff are zero in the images: their products are zero
+        fp8_silu_mul(acc[0], acc[1], acc[0]);
         float fm = kFp8Tiny;
 #pragma unroll
-        for (int j = 0; j < 64; j += 2) {
-          // rows past n_ff are zero in the images: their products are zero
-          acc[0][j] = fp8_silu_mul(acc[0][j], acc[1][j]);
-          acc[0][j + 1] = fp8_silu_mul(acc[0][j + 1], acc[1][j + 1]);
-          fm = max_abs3(fm, acc[0][j], acc[0][j + 1]);
-        }
+        for (int j = 0; j < 64; j += 2) fm = max_abs3(fm, acc[0][j], acc[0][j + 1]);
         uint32_t mx = __float_as_uint(fm);  // a NaN's bits are above every number's
         uint32_t* maxima = reinterpret_cast<uint32_t*>(smem + L::kMax);
         maxima[h * 128 + q * 32 + lane] = mx;
@@ -1216,16 +1214,16 @@ __global__ void __launch_bounds__(kJoinThreads) k_fp8_join(const __grid_constant
   }
   if constexpr (kGlu) {
     const int64_t n_ff = g.rows / 2, col = (int64_t)unit * kFp8Group + c0;
-#pragma unroll
-    for (int j = 0; j < 4; ++j) acc[j] = fp8_silu_mul(acc[j], acc[j + 4]);
-    maxima[warp * 32 + lane] = __float_as_uint(max_abs3(max_abs3(kFp8Tiny, acc[0], acc[1]), acc[2], acc[3]));
+    float o[4];
+    fp8_silu_mul({acc[0], acc[1], acc[2], acc[3]}, {acc[4], acc[5], acc[6], acc[7]}, o);
+    maxima[warp * 32 + lane] = __float_as_uint(max_abs3(max_abs3(kFp8Tiny, o[0], o[1]), o[2], o[3]));
     __syncthreads();
     uint32_t mx = 0;  // a NaN's bits are above every number's
 #pragma unroll
     for (int i = 0; i < 32; ++i) mx = max(mx, maxima[i * 32 + lane]);
     const float gm = __uint_as_float(mx), inv = fp8_inverse(gm);
     if (tok < g.m) {
-      const uint32_t w = cvt_e4m3x4(acc[0] * inv, acc[1] * inv, acc[2] * inv, acc[3] * inv);
+      const uint32_t w = cvt_e4m3x4(o[0] * inv, o[1] * inv, o[2] * inv, o[3] * inv);
       uint8_t* qrow = p.act_q + tok * p.ld_act + col;  // ld_act is a multiple of 16
       if (col + 4 <= n_ff) *reinterpret_cast<uint32_t*>(qrow) = w;
       else

@@ -13,13 +13,13 @@
 // is rounded once, to e4m3.
 //
 // Bound by HBM once there are rows enough: 16384 x 8192 bf16 with a residual 144 us
-// (6.5 TB/s, a copy's rate), 2048 x 28672 bf16 SwiGLU 47 us (6.3 TB/s).  A group is 16 or
+// (6.5 TB/s, a copy's rate), 2048 x 28672 bf16 SwiGLU 45 us (6.5 TB/s).  A group is 16 or
 // 32 neighbouring lanes' 16-byte pieces, so its maximum is a few shuffles and nothing
 // waits for another warp but a norm row's sum.  One row of 4096 takes 2.3 us, a launch's
 // latency.  Rows that do not start at multiples of 16 bytes are read by elements, at two
 // thirds of the rate, or, 16-bit norm rows, cut out of aligned 16-byte words: 16384 x
 // 8190 bf16 with a residual 278 us (by elements 400), without 150 (190).  f32 rows and the
-// other two operators are faster by elements (16384 x 8190 SwiGLU 151 us against 161,
+// other two operators are faster by elements (16384 x 8190 SwiGLU 172 us against 181,
 // 8192 x 8191 f32 with a residual 164 against 234).
 //
 // A group's maximum keeps a NaN, and an infinite one has a NaN inverse: a group
@@ -218,9 +218,10 @@ constexpr int kRowThreads = 256;
 
 // One row and 256 * kN * kV columns per CTA, or kNarrow: kN * blockDim.y rows of one piece
 // per thread (blockDim.x is a multiple of 32).  A thread requests its kN pieces of
-// every input before it uses the first.
+// every input before it uses the first.  SwiGLU is held to the registers of a full SM
+// (kN == 1) or of six CTAs: 16384 x 2048 bf16 30.0 us, 42.2 with those it would take.
 template <int kMode, typename T, bool kVec, bool kNarrow, int kN>
-__global__ void __launch_bounds__(kRowThreads) k_fp8_rows(const RowArgs g) {
+__global__ void __launch_bounds__(kRowThreads, kMode != kRowSwiglu ? 1 : kN == 1 ? 8 : 6) k_fp8_rows(const RowArgs g) {
   constexpr int kV = Vec<T>::kV;
   pdl_launch_dependents();
   pdl_wait();
@@ -245,8 +246,7 @@ __global__ void __launch_bounds__(kRowThreads) k_fp8_rows(const RowArgs g) {
       if constexpr (kMode == kRowSwiglu) {
         float u[kV];
         unpack<T>(pb[i], u);
-#pragma unroll
-        for (int j = 0; j < kV; ++j) z[j] = fp8_silu_mul(z[j], u[j]);
+        fp8_silu_mul(z, u, z);
       }
       const float gm = group_max<T>(z);
       if (c < g.k && row < g.m) {
