@@ -1255,6 +1255,23 @@ int check_device(const char* who, const AhFp8Weight* w) {
   return AH_OK;
 }
 
+// Makes a weight's device current while plans are made for it.
+struct DeviceScope {
+  int before = -1;
+  cudaError_t error;
+  explicit DeviceScope(int device) {
+    error = cudaGetDevice(&before);
+    if (error == cudaSuccess && device != before) error = cudaSetDevice(device);
+    if (error != cudaSuccess) cudaGetLastError();
+  }
+  ~DeviceScope() {
+    int now = before;
+    if (before >= 0 && cudaGetDevice(&now) == cudaSuccess && now != before) cudaSetDevice(before);
+  }
+  DeviceScope(const DeviceScope&) = delete;
+  DeviceScope& operator=(const DeviceScope&) = delete;
+};
+
 // The pairs (or single CTAs) of a launch and how its tiles are dealt out.  Splitting the tiles past
 // the last full round saves column blocks' time (about 0.45 us each) and costs a
 // launch (3 us) and the partial sums' way to L2 and back (about 6 TB/s).
@@ -1493,6 +1510,8 @@ int check_ffn(const AhFp8Weight* gate_up, const AhFp8Weight* down, int64_t m) {
   AH_REQUIRE(gate_up && down, "fp8_ffn: null weight");
   AH_REQUIRE(gate_up->gate_up && !down->gate_up && down->cols == gate_up->rows / 2 && down->rows == gate_up->cols,
              "fp8_ffn: needs a gate/up weight of 2 * n_ff rows and a down weight [n_embd][n_ff]");
+  AH_REQUIRE(gate_up->device == down->device, "fp8_ffn: the weights live on devices %d and %d", gate_up->device,
+             down->device);
   AH_REQUIRE(gate_up->nt / 2 <= 65535 && down->nt <= 65535, "fp8_ffn: more than 65535 row tiles");
   const int rc = check_matmul(gate_up, m);
   return rc != AH_OK ? rc : check_matmul(down, m);
@@ -1552,6 +1571,9 @@ int ah_fp8w_matmul_workspace_bytes(const AhFp8Weight* w, int64_t m, size_t* byte
   const int rc = check_matmul(w, m);
   if (rc != AH_OK) return rc;
   AH_REQUIRE(bytes, "fp8w_matmul_workspace_bytes: null output");
+  const DeviceScope on(w->device);  // the plan goes by the device that will run it
+  if (on.error != cudaSuccess)
+    return fail(AH_ECUDA, "fp8w_matmul_workspace_bytes: device %d: %s", w->device, cudaGetErrorString(on.error));
   *bytes = matmul_bytes(w, false, m);
   return AH_OK;
 }
@@ -1565,6 +1587,9 @@ int ah_fp8_ffn_workspace_bytes(const AhFp8Weight* gate_up, const AhFp8Weight* do
   const int rc = check_ffn(gate_up, down, m);
   if (rc != AH_OK) return rc;
   AH_REQUIRE(bytes, "fp8_ffn_workspace_bytes: null output");
+  const DeviceScope on(down->device);
+  if (on.error != cudaSuccess)
+    return fail(AH_ECUDA, "fp8_ffn_workspace_bytes: device %d: %s", down->device, cudaGetErrorString(on.error));
   *bytes = ffn_layout(gate_up, down, m).total;
   return AH_OK;
 }

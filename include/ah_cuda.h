@@ -580,7 +580,8 @@ AH_API int64_t ah_fp8w_weight_bytes(const AhFp8Weight* w);
  * inference/math.rs:255-295 gemv_4bit_into for m tokens.  y [m][ldy], ldy >= rows.
  * The workspace (16-byte aligned, any contents, ah_fp8w_matmul_workspace_bytes, 0
  * for many shapes) takes the partial sums of tiles split along the columns and
- * serves one call at a time; with workspace null nothing is split, which is slower
+ * serves one call at a time (its size is planned for the weight's device, whichever is
+ * current); with workspace null nothing is split, which is slower
  * where bytes were asked for and adds in another order. */
 AH_API int ah_fp8w_matmul_workspace_bytes(const AhFp8Weight* w, int64_t m, size_t* bytes);
 AH_API int ah_fp8w_matmul(const AhFp8Weight* w, const uint8_t* q_dev, int64_t ldq, const float* scales_dev,
