@@ -69,7 +69,7 @@ def _quantised(q: torch.Tensor, scales: torch.Tensor, m: int, k: int, device: in
     if q.dtype is not _E4M3 or scales.dtype is not _F32:
         _refuse("expected q as float8_e4m3fn and scales as float32")
     ldq, lds = _like(q, m, k, device, "q"), _like(scales, m, (k + 127) // 128, device, "scales")
-    return (ldq + 15) // 16 * 16 if m == 1 else ldq, lds
+    return (ldq + 15) // 16 * 16 if m <= 1 else ldq, lds  # the stride of one row or none is free
 
 
 def alloc(m: int, k: int, device="cuda") -> tuple[torch.Tensor, torch.Tensor]:

@@ -1,0 +1,15 @@
+"""CPU: the 8-bit floating point front-end's own rules, on tensors without a device."""
+import pytest
+
+from agent_harness_b200 import fp8
+
+CPU = -1  # what Tensor.get_device() gives
+
+
+@pytest.mark.parametrize("k", [1, 16, 100, 1003])
+@pytest.mark.parametrize("m", [0, 1, 3])
+def test_row_strides_of_any_batch(m, k):
+    """alloc's pairs pass their own check with a row stride of whole 16-byte pieces; torch
+    calls a matrix of one row or none contiguous, whatever its stride."""
+    ldq, lds = fp8._quantised(*fp8.alloc(m, k, "cpu"), m, k, CPU)
+    assert ldq == (k + 15) // 16 * 16 and lds == (k + 127) // 128
