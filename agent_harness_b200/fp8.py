@@ -244,7 +244,7 @@ class Fp8SwigluBlock:
 
     @staticmethod
     def _check(gate, up, down):
-        if gate.shape != up.shape or down.shape != (gate.shape[1], gate.shape[0]):
+        if gate.dim() != 2 or gate.shape != up.shape or down.shape != (gate.shape[1], gate.shape[0]):
             _refuse("expected gate and up [n_ff, n_embd] and down [n_embd, n_ff]")
         if not (gate.device == up.device == down.device and gate.dtype == up.dtype):
             _refuse("gate, up and down must be on one device, gate and up of one type")
