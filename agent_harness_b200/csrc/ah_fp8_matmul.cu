@@ -445,6 +445,14 @@ __global__ void __launch_bounds__(kSmallThreads, 2) k_fp8_small(const __grid_con
         ph ^= 1;
       }
     }
+    // the last releases arrive, too, before the CTA can exit
+    for (int i = 0; i < ahead; ++i) {
+      wait_bar(&empty[r], ph, p.err, abort_flag);
+      if (++r == L::kStages) {
+        r = 0;
+        ph ^= 1;
+      }
+    }
     if (*abort_flag)  // the copies in flight land before the CTA can exit
       for (int s = max(0, n_stage - L::kStages); s < n_stage; ++s)
         mbar_wait_bounded(&full[s % L::kStages], (uint32_t)((s / L::kStages) & 1), p.err, AH_ETIMEOUT, 1u << 12);
@@ -917,6 +925,9 @@ __global__ void __launch_bounds__(kBigThreads, 1) k_fp8_big(const __grid_constan
           }
         }
       }
+      // the last releases, which the leader sends to both CTAs, arrive before either can exit
+      for (int i = 0; i < L::kStages; ++i)
+        wait_bar(&empty[(s + i) % L::kStages], s + i < L::kStages ? ph : ph ^ 1, p.err, abort_flag);
       if (*abort_flag && rank == 0)  // the copies in flight land before the pair can exit
         for (int i = 0; i < L::kStages; ++i)
           mbar_wait_bounded(&full[i], i < s ? ph ^ 1 : ph, p.err, AH_ETIMEOUT, 1u << 12);
@@ -953,7 +964,10 @@ __global__ void __launch_bounds__(kBigThreads, 1) k_fp8_big(const __grid_constan
           dph ^= buf == 0;
         }
       if (*abort_flag) {  // the MMAs in flight end before the tensor memory is freed
-        if (elected) commit(drained);
+        if (elected) {  // an arrival in this CTA alone: the other one does not wait for it
+          if constexpr (kPair) mma_commit_pair_self(drained);
+          else mma_commit(drained);
+        }
         mbar_wait_bounded(drained, 0, p.err, AH_ETIMEOUT, kWaitLimit);
       }
     }

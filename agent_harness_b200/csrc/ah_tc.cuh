@@ -102,6 +102,11 @@ __device__ __forceinline__ void mma_commit_pair(uint64_t* bar) {
       "h"((uint16_t)3)
       : "memory");
 }
+// The same for a barrier of the issuing CTA alone.
+__device__ __forceinline__ void mma_commit_pair_self(uint64_t* bar) {
+  asm volatile("tcgen05.commit.cta_group::2.mbarrier::arrive::one.shared::cluster.b64 [%0];" ::"r"(smem_u32(bar))
+               : "memory");
+}
 // A TMA load into this CTA that completes on a barrier of the pair (a
 // shared::cluster address, e.g. the leader's).
 __device__ __forceinline__ void tma_load_2d_pair(uint32_t dst, const void* tmap, int x, int y, uint32_t bar) {
