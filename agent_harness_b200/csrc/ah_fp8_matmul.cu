@@ -461,6 +461,7 @@ __global__ void __launch_bounds__(kSmallThreads, 2) k_fp8_small(const __grid_con
     constexpr uint32_t idesc = idesc_e4m3(128, kNt);
     int r = 0, buf = 0;
     uint32_t ph = 0, dph = 1;  // the buffers start empty
+    pdl_wait();  // here, too: the waits for the tokens are counted from the end of the preceding grid
     for (int i = 0; i < nb; ++i) {
       if (i % L::kKs == 0) wait_bar(&full[r], ph, p.err, abort_flag);
       wait_bar(&d_empty[buf], dph, p.err, abort_flag);
@@ -940,6 +941,7 @@ __global__ void __launch_bounds__(kBigThreads, 1) k_fp8_big(const __grid_constan
       };
       int s = 0, buf = 0;
       uint32_t ph = 0, dph = 1;  // the buffers start empty
+      pdl_wait();  // here, too: the waits for the tokens are counted from the end of the preceding grid
       while (walk.next(p.split, kb))
         for (int b = walk.b0; b < walk.b1; ++b) {
           wait_bar(&full[s], ph, p.err, abort_flag);
