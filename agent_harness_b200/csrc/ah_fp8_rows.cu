@@ -219,9 +219,9 @@ constexpr int kRowThreads = 256;
 // One row and 256 * kN * kV columns per CTA, or kNarrow: kN * blockDim.y rows of one piece
 // per thread (blockDim.x is a multiple of 32).  A thread requests its kN pieces of
 // every input before it uses the first.  SwiGLU is held to the registers of a full SM
-// (kN == 1) or of six CTAs: 16384 x 2048 bf16 30.0 us, 42.2 with those it would take.
+// (kN == 1) or of six CTAs: 16384 x 2048 bf16 30.0 us, 33.8 with those it would take.
 template <int kMode, typename T, bool kVec, bool kNarrow, int kN>
-__global__ void __launch_bounds__(kRowThreads, kMode != kRowSwiglu ? 1 : kN == 1 ? 8 : 6) k_fp8_rows(const RowArgs g) {
+__global__ void __launch_bounds__(kRowThreads, kMode != kRowSwiglu ? 0 : kN == 1 ? 8 : 6) k_fp8_rows(const RowArgs g) {
   constexpr int kV = Vec<T>::kV;
   pdl_launch_dependents();
   pdl_wait();
