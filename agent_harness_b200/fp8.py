@@ -7,7 +7,11 @@ A quantised matrix is a pair (q, scales): q [m, k] torch.float8_e4m3fn whose row
 start at multiples of 16 bytes (alloc gives such a pair; so does every call here),
 scales [m, ceil(k / 128)] f32.  Everything runs on torch's current stream of the
 inputs' device, allocates through torch only, and can be captured into a CUDA
-graph once a weight has been made."""
+graph once a weight has been made.
+
+The products' waits on the device are bounded.  A call whose wait gives up leaves its
+outputs unwritten and sets the library's device error word, which no call here reads, since
+that would wait for the stream: lib().ah_check_device_error(stream) does, and clears it."""
 from __future__ import annotations
 
 import ctypes as C

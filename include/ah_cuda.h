@@ -535,11 +535,15 @@ AH_API int ah_ssm_forward(const AhSsmConfig* cfg, const AhSsmWeights* w, float* 
  *
  * With g = max(max |z|, 2^-100) over the group: q = e4m3(z * (448 / g)) rounded to
  * nearest even, scale = g / 448.  A group that holds a NaN or an infinity stands for
- * NaN throughout. */
+ * NaN throughout.
+ *
+ * The products' waits on the device are bounded: one that gives up leaves outputs
+ * unwritten and is reported by ah_check_device_error alone. */
 /* z = x. */
 AH_API int ah_fp8_quantize(const void* x_dev, int64_t ldx, uint32_t dtype, int64_t m, int64_t k, uint8_t* q_dev,
                            int64_t ldq, float* scales_dev, int64_t lds, void* stream);
-/* z = silu(gate) * up, the activation of inference/ffn.rs:155-174, in f32. */
+/* z = silu(gate) * up, the activation of inference/ffn.rs:155-174, in f32; it keeps its
+ * value where exp(-gate) passes the largest f32, and is 0 below a gate of -173.9. */
 AH_API int ah_fp8_swiglu(const void* gate_dev, int64_t ld_gate, const void* up_dev, int64_t ld_up, uint32_t dtype,
                          int64_t m, int64_t k, uint8_t* q_dev, int64_t ldq, float* scales_dev, int64_t lds,
                          void* stream);
