@@ -71,3 +71,38 @@ def test_huge_gates(fp8, dtype):  # noqa: F811
     x = (x * torch.where(torch.rand_like(x) < 0.5, -1.0, 1.0)).to(dtype)
     q, s = fp8.swiglu_fp8(x, torch.full_like(x, 2.0**-9))
     assert torch.isfinite(s).all() and torch.isfinite(q.float()).all()
+
+
+@pytest.mark.parametrize("m,n_embd,n_ff", [(1, 512, 1100), (20, 256, 700), (130, 384, 700), (100, 256, 12900), (400, 700, 2500), (320, 8192, 2000)])
+def test_block_with_far_gates(fp8, m, n_embd, n_ff):  # noqa: F811
+    """Every kernel of the block: gates of about -30, -86, -88, -89, -110 and -150 by tiles of
+    128, ups of 1e25 and more, and outputs that see one tile each.  Against the block's
+    steps: the activations may sit one e4m3 step (2^-3) apart where a last bit differs."""
+    tiles, kb = (n_ff + 127) // 128, (n_embd + 127) // 128
+    x = 1 + 0.1 * randn(m, n_embd, seed=1).clamp(-2, 2)  # normalised: about 1 everywhere
+    w = torch.ones(n_embd, device="cuda")
+    gate = torch.tensor([-30.0, -86.2, -88.0, -89.0, -110.0, -150.0], device="cuda")[torch.arange(tiles, device="cuda") % 6]
+    gq = torch.full((n_ff, n_embd), 1.0, device="cuda").to(torch.float8_e4m3fn)
+    gs = (gate / n_embd)[:, None].repeat(1, kb)
+    uq = randn(n_ff, n_embd, seed=2).clamp(-4, 4).to(torch.float8_e4m3fn)
+    us = torch.full((tiles, kb), 1e25, device="cuda") * torch.exp2(torch.arange(tiles, device="cuda") % 6 * 4.0)[:, None]
+    tile_of = torch.arange(n_embd, device="cuda")[:, None] % tiles == torch.arange(n_ff, device="cuda")[None] // 128
+    dq = (randn(n_embd, n_ff, seed=3).clamp(-4, 4) * tile_of).to(torch.float8_e4m3fn)
+    ds = torch.full((kb, tiles), 2.0**-4, device="cuda")
+    block = fp8.Fp8SwigluBlock.from_blocks(gq, gs, uq, us, dq, ds)
+    y = block(x, w)
+    q, s = fp8.add_rms_norm_fp8(x, w)
+    gu = block.gate_up.matmul(q, s)
+    assert (gu[:, :n_ff] < -25).all() and (gu[:, :n_ff].amin() < -100 if tiles > 4 else True)
+    a, asc = fp8.swiglu_fp8(gu[:, :n_ff], gu[:, n_ff:])
+    check(a, asc, swiglu(gu[:, :n_ff], gu[:, n_ff:]))
+    want = block.down.matmul(a, asc)
+    seen = (torch.arange(n_embd, device="cuda") % tiles) % 6 != 5  # -150: below the smallest group's scale
+    assert torch.isfinite(y).all()
+    step = a.float().abs().clamp(min=2.0**-6) * 2.0**-3 * asc.repeat_interleave(G, 1)[:, :n_ff]
+    bound = step.double() @ (dq.double().abs() * 2.0**-4).t() + 2.0**-16 * want.abs().double() + 1e-30
+    assert ((y.double() - want.double()).abs() <= bound).all()
+    assert (y[:, seen].double() - want[:, seen]).norm() <= 2.0**-8 * want[:, seen].norm()
+    per_tile = y.abs().amax(0)
+    assert (per_tile[seen] > 0).all()
+    block.close()
