@@ -299,10 +299,11 @@ __device__ __forceinline__ void store_swiglu4(const Args& p, int64_t token, int6
 // Bound by the weight stream (a token costs it nothing up to 32): the first stages'
 // weights are requested before the kernel waits for the grid ahead of it (a weight
 // is complete once its handle exists), and two CTAs per SM keep 200 KB in flight.
-// 128256 x 4096 at 16 tokens 87 us (6.1 TB/s), 28672 x 8192 at one 39 us (6.0), 4096 x
-// 4096 at one 5.7 us (3.0: launch, first copies and the cluster's sum take 3 us).  At
+// 128256 x 4096 at 16 tokens 85 us (6.3 TB/s), 28672 x 8192 at one 37 us (6.3), 4096 x
+// 4096 at one 6.0 us (2.8: launch, first copies and the cluster's sum take 3 us).  At
 // 64 tokens the shared memory's bandwidth is the bound (operands twice, and a
-// broadcast read of four scales per four columns): 14336 x 4096 16.3 us (3.8 TB/s).
+// broadcast read of four scales per four columns): 14336 x 4096 15.9 us (3.7 TB/s).
+// Times in this file: calls captured back to back, inputs past the L2, a cool GPU.
 
 constexpr uint32_t kWaitLimit = 1u << 24;
 constexpr int kSmallThreads = 192;
@@ -701,17 +702,17 @@ int dispatch_small(SmallArgs& p, cudaStream_t st) {
 // loading both images (48 KB per column block, M = 128): half of a pair's rows would be
 // empty.  A tile's column blocks are shared by a cluster of two, four or eight where
 // that many fit the GPU at once; its members add their sums through distributed shared
-// memory in rank order (65 x 6144 x 4096 12.7 us, by partial sums in global memory and a
-// second launch 14.5; 65 x 8192 x 8192 19.0 against 20.8; requesting several tokens' sums
-// at a time was no faster).  128 x 28672 x 8192 45 us (5.2 TB/s of weights; pairs 66), 128 x 32000 x 2048
-// 16.7 (24), a 4096 x 14336 feed-forward block at 128 tokens 53 (65).  Past 128 tokens
-// single CTAs load half as much again: 443 us where pairs take 414.
+// memory in rank order (65 x 6144 x 4096 12.6 us, by partial sums in global memory and a
+// second launch 14.5; 65 x 8192 x 8192 18.5 against 19.6; requesting several tokens' sums
+// at a time was no faster).  128 x 28672 x 8192 45 us (5.2 TB/s of weights; pairs 65), 128 x 32000 x 2048
+// 16.4 (21.9), a 4096 x 14336 feed-forward block at 128 tokens 51 (69).  Past 128 tokens
+// single CTAs load half as much again (2048 x 28672 x 8192 443 us where pairs took 414).
 //
 // What bounds it: a column block's MMAs take 560 cycles, and a buffer's way round
 // (MMAs, the commit's way to both CTAs, the readers, their arrivals' way back) 1700 to
-// 1800, hidden by two buffers down to 850 to 900.  2048 x 28672 x 8192 takes 414 us (2322
-// TFLOP/s; sustained, the power cap leaves 2000).  Readers that only read tensor memory
-// leave 373 us, that only multiply and add 406, that hand the buffers back at once 333
+// 1800, hidden by two buffers down to 850 to 900.  2048 x 28672 x 8192 takes 403 to 420 us
+// by the card (2290 to 2390 TFLOP/s; sustained, the power cap leaves 2000).  On one of 414,
+// readers that only read tensor memory leave 373 us, that only multiply and add 406, that hand the buffers back at once 333
 // and 570 cycles.  Measured and not kept: half buffers of N = 128 (452 us) and tiles of
 // one weight tile with four buffers (506), both bound by the readers' fixed cost per
 // wait; scales through shared memory (427); paired multiply-adds (fma.f32x2, 561: their
@@ -1415,11 +1416,12 @@ int launch_big(BigArgs& p, const BigPlan& plan, cudaStream_t st) {
 
 // Whether a product goes to k_fp8_big.  The weight-streaming kernel
 // takes up to 32, and 33 to 64 while the tiles of single CTAs would leave a third of the
-// SMs idle (64 tokens: 14336 x 4096 17.7 us against 19.0, but 28672 x 8192 49 against
-// 43, a 4096 x 14336 feed-forward block 50 with its gate/up product there against 44).  It takes more while its tiles, one per 64 tokens (32 for a gate/up pair), leave
-// clusters of four (two) on two CTAs per SM: 4096 x 4096 at 128 tokens 12.0 us against
-// 14.2 of single CTAs, but at 192 15.0 against 13.7 of pairs, and 8192 x 512 at 128 7.2
-// against 6.1.
+// SMs idle (64 tokens: 14336 x 4096 15.9 us against 17.4, but 28672 x 8192 45.5 against
+// 42.5, a 4096 x 14336 feed-forward block 54 with its gate/up product there against 44).
+// It takes more while its tiles, one per 64 tokens (32 for a gate/up pair), leave
+// clusters of four (two) on two CTAs per SM: 4096 x 4096 at 128 tokens 10.7 us against
+// 13.6 of single CTAs, but at 192 15.1 against 14.0 of pairs, and 8192 x 512 at 128 7.4
+// against 6.5.
 bool use_big(const AhFp8Weight* w, bool glu, int64_t m) {
   if (m <= 32) return false;
   if (m <= 64) return (w->nt + 1) / 2 * 3 > sm_count() * 2;

@@ -15,12 +15,15 @@
 // Bound by HBM once there are rows enough: 16384 x 8192 bf16 with a residual 144 us
 // (6.5 TB/s, a copy's rate), 2048 x 28672 bf16 SwiGLU 45 us (6.5 TB/s).  A group is 16 or
 // 32 neighbouring lanes' 16-byte pieces, so its maximum is a few shuffles and nothing
-// waits for another warp but a norm row's sum.  One row of 4096 takes 2.3 us, a launch's
-// latency.  Rows that do not start at multiples of 16 bytes are read by elements, at two
-// thirds of the rate, or, 16-bit norm rows, cut out of aligned 16-byte words: 16384 x
-// 8190 bf16 with a residual 278 us (by elements 400), without 150 (190).  f32 rows and the
-// other two operators are faster by elements (16384 x 8190 SwiGLU 172 us against 181,
-// 8192 x 8191 f32 with a residual 164 against 234).
+// waits for another warp but a norm row's sum.  One row of 4096 takes 2.4 us, a launch's
+// latency.  Without a residual the norm's arithmetic, the same for half the bytes, is the
+// bound: 16384 x 8192 bf16 89 us (4.5 TB/s), 77 % of issue slots busy.
+//
+// Rows that do not start at multiples of 16 bytes are read by elements, at two thirds of
+// the rate, or, 16-bit norm rows, cut out of aligned 16-byte words: 16384 x 8190 bf16 with a
+// residual 276 us (by elements 400), without 149 (190).  f32 rows and the other two
+// operators are faster by elements (16384 x 8190 SwiGLU 172 us against 181, 8192 x 8191 f32
+// with a residual 164 against 234).
 //
 // A group's maximum keeps a NaN, and an infinite one has a NaN inverse: a group
 // with a NaN or an infinity comes out as NaN.
@@ -417,8 +420,9 @@ int launch_rows(const RowArgs& g, bool vec, cudaStream_t st) {
   vec = vec && g.k % Vec<T>::kV == 0;
   if (pieces <= kRowThreads) {
     // Narrow rows share a CTA, and a thread takes a piece of kRows rows once that leaves every
-    // SM four CTAs.  16384 x 2048 bf16 quantise: 18.1 us with four, 19.9 with two, 24.7 with
-    // one; 16384 x 1024 f32 SwiGLU 25.4, 24.6, 27.1; 16384 x 2048 bf16 SwiGLU 35.1, 32.7, 29.0.
+    // SM four CTAs.  16384 x 2048 bf16 quantise: 18.8 us with four, 20.8 with two, 24.6 with
+    // one; 16384 x 1024 f32 SwiGLU 29.8, 23.3, 24.3; bf16 SwiGLU 16384 x 2048 39.7, 29.2, 30.0,
+    // 16384 x 512 14.6, 9.2, 9.0.
     constexpr int kRows = kMode == kRowQuantize ? 4 : sizeof(T) == 4 ? 2 : 1;
     const unsigned tx = (unsigned)((pieces + 31) / 32 * 32), ty = kRowThreads / tx;
     const bool many = vec && g.m >= (int64_t)kRows * ty * 4 * sm_count();
@@ -429,7 +433,7 @@ int launch_rows(const RowArgs& g, bool vec, cudaStream_t st) {
                       grid, dim3(tx, ty), 0, st, g);
   }
   // Wide ones take two pieces per thread once that still leaves every SM four CTAs
-  // (16384 x 8192 bf16 SwiGLU: 104 us with two, 120 with one).
+  // (16384 x 8192 bf16 SwiGLU: 100 us with two, 117 with one).
   const bool many = vec && g.m * ((pieces + 2 * kRowThreads - 1) / (2 * kRowThreads)) >= 4 * (int64_t)sm_count();
   const int64_t cols = (int64_t)kRowThreads * (many ? 2 : 1);
   const dim3 grid((unsigned)((pieces + cols - 1) / cols), (unsigned)std::min<int64_t>(g.m, 65535));
@@ -450,8 +454,8 @@ int launch_norm(const NormArgs& g, bool vec, cudaStream_t st) {
   // Few rows: one piece per thread, up to 1024 threads, for the latency of one
   // round of loads.  Many rows: few threads per row and many pieces each, so that a
   // row's sum costs little and many rows are in flight (16384 x 8192 bf16 with a
-  // residual: 151 us with four pieces, 190 with two, 321 with one); without the
-  // residual's registers, eight.
+  // residual: 144 us with four pieces, 199 with eight, 169 with two, 271 with one); without
+  // the residual's registers, eight (89 us, with four 95).
   constexpr int kMany = kRes ? 4 : 8;
   const int64_t pieces = (g.k + Vec<T>::kV - 1) / Vec<T>::kV;
   vec = vec && g.k % Vec<T>::kV == 0;
