@@ -161,6 +161,10 @@ int build(const TileSource (&s)[2], int kind, bool gate_up, int64_t rows, int64_
     AH_REQUIRE(kind == kSourceE4m3 ? element_aligned(s[i].scales, AH_DTYPE_F32) : element_aligned(s[i].p, kind == kSourceF32 ? AH_DTYPE_F32 : AH_DTYPE_F16),
                "fp8w: a source is not aligned to its elements");
   }
+  // an allocation, or the wait below, would end the capture
+  cudaStreamCaptureStatus capture = cudaStreamCaptureStatusNone;
+  if (cudaStreamIsCapturing(st, &capture) != cudaSuccess) cudaGetLastError();  // no device: the allocation says so
+  AH_REQUIRE(capture == cudaStreamCaptureStatusNone, "fp8w: a weight cannot be made on a capturing stream");
   AhFp8Weight* w = new (std::nothrow) AhFp8Weight();
   if (!w) return fail(AH_ENOMEM, "fp8w: out of host memory");
   w->rows = gate_up ? 2 * rows : rows;

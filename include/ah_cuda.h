@@ -559,7 +559,7 @@ AH_API int ah_fp8_add_rms_norm(const void* x_dev, int64_t ldx, void* residual_de
 /* Opaque device-resident weight [rows][cols]: e4m3 and one f32 scale per
  * 128 x 128 block, in the tensor cores' tile order, on the device that was current
  * when it was made.  The makers copy their sources, wait for `stream` and so
- * cannot be captured. */
+ * refuse a capturing one (the capture goes on). */
 typedef struct AhFp8Weight AhFp8Weight;
 /* q [rows][ldq] e4m3 bytes (any ldq >= cols), scales [ceil(rows/128)][lds >= ceil(cols/128)]. */
 AH_API int ah_fp8w_from_blocks(const uint8_t* q_dev, int64_t ldq, const float* scales_dev, int64_t lds, int64_t rows,
