@@ -716,13 +716,13 @@ int dispatch_small(SmallArgs& p, cudaStream_t st) {
 // (MMAs, the commit's way to both CTAs, the readers, their arrivals' way back) 1700 to
 // 1800, hidden by two buffers down to 850 to 900.  2048 x 28672 x 8192 takes 403 to 420 us
 // by the card (2290 to 2390 TFLOP/s; sustained, the power cap leaves 2000).  On one of 414,
-// readers that only read tensor memory leave 373 us, that only multiply and add 406, that hand the buffers back at once 333
-// and 570 cycles.  Measured and not kept: half buffers of N = 128 (452 us) and tiles of
-// one weight tile with four buffers (506), both bound by the readers' fixed cost per
-// wait; scales through shared memory (427); paired multiply-adds (fma.f32x2, 561: their
-// register pairs spill).  A release of cluster scope on the arrivals cost a memory
-// barrier each (939 against 598 us at the time), issuing copies and MMAs outside uniform
-// code another third.
+// readers that only read tensor memory leave 373 us, that only multiply and add 406, that
+// hand the buffers back at once 333 and 570 cycles.  Measured and not kept: half buffers of
+// N = 128 (452 us) and tiles of one weight tile with four buffers (506), both bound by the
+// readers' fixed cost per wait; scales through shared memory (427); paired multiply-adds
+// (fma.f32x2, 561: their register pairs spill).  A release of cluster scope on the arrivals
+// cost a memory barrier each (939 against 598 us at the time), issuing copies and MMAs
+// outside uniform code another third.
 
 constexpr int kBigThreads = 384;
 // Registers: 384 threads start with 168 each (64512); the first four warps drop
