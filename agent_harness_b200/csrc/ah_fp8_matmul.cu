@@ -785,7 +785,7 @@ struct BigArgs {
   CUtensorMap tm_w;  // weight images as bytes [images * 128][128], box 128 x 128
   CUtensorMap tm_y;  // y [m][rows], box 128 bytes x 32 rows, 128-byte swizzle (when y_map)
   MatmulArgs g;
-  bool y_map;
+  bool y_map, y_whole;  // y has a map; its rows are whole 16-byte pieces, which a tiled store writes
   bool cluster;  // single CTAs: a split tile's parts are a cluster and add their sums in it
   BigSplit split;
   float* partial;
@@ -1111,7 +1111,7 @@ __global__ void __launch_bounds__(kBigThreads, 1) k_fp8_big(const __grid_constan
         }
       } else if (!ok) {
         continue;
-      } else if (p.y_map) {
+      } else if (p.y_map && (p.y_whole || (int64_t)(unit + 1) * 2 * kFp8Group <= g.rows)) {
         // 128-byte rows through the warp's 4 KB stage (16-byte pieces swizzled as
         // the map does), one tiled store per 32 rows
         const bool wide = g.y_dtype == AH_DTYPE_F32;
@@ -1146,10 +1146,11 @@ __global__ void __launch_bounds__(kBigThreads, 1) k_fp8_big(const __grid_constan
           }
         }
       } else {
-        // y that no tensor map can address: 32 x 32 f32 boxes through the warp's
-        // stage, each token's 32 columns written by the whole warp
+        // y that no tensor map can address, or rows that end inside a 16-byte piece: 32 x 32
+        // f32 boxes through the warp's stage, each token's 32 columns written by the whole warp
         const int64_t rows = g.gate_up ? g.rows / 2 : g.rows;  // rows of a tile's source
         float* box = reinterpret_cast<float*>(stage);
+        if (lane == 0) bulk_wait_read0();  // another tile's last store has read the stage
 #pragma unroll
         for (int c = 0; c < 4; ++c) {
           __syncwarp();
@@ -1370,6 +1371,7 @@ int launch_big(BigArgs& p, const BigPlan& plan, cudaStream_t st) {
   if (rc != AH_OK) return rc;
   const int elem = g.y_dtype == AH_DTYPE_F32 ? 4 : 2;
   p.y_map = !kGlu && !g.gate_up && aligned16(g.y) && g.ldy * elem % 16 == 0;
+  p.y_whole = g.rows * elem % 16 == 0;
   if (p.y_map) {
     const CUtensorMapDataType dt = elem == 4 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT32 : CU_TENSOR_MAP_DATA_TYPE_UINT16;
     auto fn = tensor_map_encoder();

@@ -122,8 +122,9 @@ __device__ __forceinline__ void tma_load_2d_pair(uint32_t dst, const void* tmap,
 __device__ __forceinline__ void mbar_arrive_cluster(uint32_t bar) {
   asm volatile("mbarrier.arrive.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
 }
-// A tiled store shared -> global (one bulk group per commit), clipped to the
-// map's extents.
+// A tiled store shared -> global (one bulk group per commit), clipped to the map's
+// extents, of the innermost one in whole 16-byte pieces: a row that ends inside a piece has
+// the rest of it written, too (seen on B200: up to 14 bytes past rows of 2-byte elements).
 __device__ __forceinline__ void tma_store_2d(const void* tmap, int x, int y, uint32_t src) {
   asm volatile("cp.async.bulk.tensor.2d.global.shared::cta.tile.bulk_group [%0, {%1, %2}], [%3];" ::"l"(tmap),
                "r"(x), "r"(y), "r"(src)

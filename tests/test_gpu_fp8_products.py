@@ -72,6 +72,22 @@ def test_poison_around_the_inputs(fp8, m, n):  # noqa: F811
         assert (y[:, :off] == -3).all() and (y[:, off + n:] == -3).all()
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("m", [1, 20, 50, 100, 300, 1648])
+@pytest.mark.parametrize("n", [1497, 1498, 1499, 1500, 1501, 1502, 1503, 20001])
+def test_neighbours_of_ragged_outputs(fp8, m, n):  # noqa: F811
+    """Rows that end inside a 16-byte piece of a wider matrix whose rows start at such
+    pieces: the rest of the piece belongs to someone else."""
+    wq, ws = blocks(n, 160, 3)
+    W = fp8.Fp8Weight.from_blocks(wq, ws)
+    q, s = acts(fp8, m, 160, 2)
+    for dtype in TYPES:
+        y = torch.full((m + 2, (n + 15) // 8 * 8 + 8), -3.0, dtype=dtype, device="cuda")
+        W.matmul(q, s, out=y[:m, :n])
+        assert (y[:, n:] == -3).all() and (y[m:] == -3).all()
+        check_product(y[:m, :n], q, s, wq, ws)
+
+
 # 16800 tokens over a vocabulary of 128256: 2^31 elements end inside row 16744.  128 tokens
 # over 16.8 million rows: output and weight pass 2^31 elements.
 HUGE = [(16800, 128256, 128, 128256), (16800, 128256, 128, 128257), (128, 16800000, 128, 16800000)]
