@@ -581,7 +581,8 @@ AH_API int ah_fp8w_shape(const AhFp8Weight* w, int64_t* rows, int64_t* cols);
 AH_API int64_t ah_fp8w_weight_bytes(const AhFp8Weight* w);
 /* y[i][r] = sum over blocks b of 128 columns of scales[i][b] * w_scale[r / 128][b] *
  * (sum over the block of q[i][j] * w[r][j]), sums in f32, rounded once to y_dtype:
- * inference/math.rs:255-295 gemv_4bit_into for m tokens.  y [m][ldy], ldy >= rows.
+ * inference/math.rs:255-295 gemv_4bit_into for m tokens.  y [m][ldy], ldy >= rows;
+ * nothing past column rows is written.  Up to 32 tokens take 65535 * 128 rows at most.
  * The workspace (16-byte aligned, any contents, ah_fp8w_matmul_workspace_bytes, 0
  * for many shapes) takes the partial sums of tiles split along the columns and
  * serves one call at a time (its size is planned for the weight's device, whichever is
