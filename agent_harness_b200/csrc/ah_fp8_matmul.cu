@@ -142,7 +142,12 @@ void destroy(AhFp8Weight* w) {
   int cur = 0;
   cudaGetDevice(&cur);
   cudaSetDevice(w->device);
+  // a handle may be collected while its thread captures something else: the free, which
+  // is no part of that, would end the capture in its usual mode
+  cudaStreamCaptureMode mode = cudaStreamCaptureModeRelaxed;
+  cudaThreadExchangeStreamCaptureMode(&mode);
   cudaFree(w->tiles);
+  cudaThreadExchangeStreamCaptureMode(&mode);
   cudaSetDevice(cur);
   delete w;
 }

@@ -27,3 +27,22 @@ def test_makers_refuse_a_capturing_stream(fp8):  # noqa: F811
     graph.replay()
     torch.cuda.synchronize()
     assert torch.equal(y, want)
+
+
+def test_a_weight_may_go_during_a_capture(fp8):  # noqa: F811
+    """Closed, or collected, while its thread captures something else: it is freed, and the
+    capture goes on."""
+    W, old = fp8.Fp8Weight.from_float(randn(256, 256)), fp8.Fp8Weight.from_float(randn(16384, 16384))
+    q, s = fp8.quantize_fp8(randn(4, 256, seed=2))
+    want, y = W.matmul(q, s), torch.zeros(4, 256, device="cuda")
+    torch.cuda.synchronize()
+    torch.cuda.empty_cache()
+    free = torch.cuda.mem_get_info()[0]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        old.close()
+        W.matmul(q, s, out=y)
+    graph.replay()
+    torch.cuda.synchronize()
+    assert torch.equal(y, want)
+    assert torch.cuda.mem_get_info()[0] > free + 200 * 2**20  # 256 MB less what the capture took
